@@ -116,6 +116,11 @@ zr_status zr_upload_globals(zr_context* ctx, const uint16_t* embedding /* [vocab
 zr_status zr_kv_pool_create(zr_context* ctx, int n_pages);
 int zr_kv_pool_pages(const zr_context* ctx);
 uint64_t zr_kv_pool_bytes(const zr_context* ctx);
+/* Device address of the pool (NULL before zr_kv_pool_create; valid until the
+ * pool is re-created or the context destroyed): [num_layers][n_pages][page
+ * bytes], a page in the pool's own order, zr_kv_pool_bytes in all.  For
+ * programs that move whole pages themselves (a peer copy, a checker). */
+void* zr_kv_pool_data(const zr_context* ctx);
 
 /* ------------------------------------------------------- microbatches --- */
 /* One ragged microbatch: decode rows (q_len 1) and prefill chunks (q_len > 1)
@@ -326,6 +331,16 @@ size_t zr_transfer_cached_bytes(const zr_context* ctx);
 zr_status zr_kv_export_cbor(zr_context* ctx, const int* block_table, int n_pages, int first_offset, int first_row,
                             int n_rows, long long base_position, int cfg_max_seq_len, uint8_t* out, size_t capacity,
                             size_t* out_len);
+/* Copies pages inside the pool: in every layer, page dst[i] becomes a copy of
+ * page src[i], i < n (host arrays, read before the call returns).  src may
+ * name a page several times; a page that is the target of two copies, or is
+ * both read and written, is ZR_E_INVALID, one outside the pool
+ * ZR_E_INVARIANT, and nothing is copied then.  The _async form enqueues the
+ * copies on the context stream.  No reference counterpart: its sessions never
+ * share pages (forward_pass.rs:250-460).  Sessions fork and compact through
+ * it (zrh_fork, zrh_pool_compact). */
+zr_status zr_kv_copy_pages(zr_context* ctx, const int* src, const int* dst, int n);
+zr_status zr_kv_copy_pages_async(zr_context* ctx, const int* src, const int* dst, int n);
 /* Raw page access for bit-exact checks: copies `n_pages` pages of `layer`
  * (K then V, pool dtype, pool layout) into host memory. */
 zr_status zr_kv_read_pages(zr_context* ctx, int layer, const int* pages, int n_pages, void* dst);

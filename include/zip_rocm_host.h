@@ -120,6 +120,38 @@ void zrh_clear(zrh_backend* b);
  * back to the pool; the session restarts empty at position 0. */
 zr_status zrh_release_pages(zrh_backend* b);
 
+/* ------------------------------------------------- shared and spare pages --- */
+/* No counterparts in the reference, whose sessions own their pages
+ * (forward_pass.rs:250-460): several continuations of one prompt (samples,
+ * beams, a common system prompt) without a copy of its window each.
+ *
+ * `child` becomes a second session with the parent's window and position; what
+ * it held goes back to the pool (zrh_release_pages).  Both sessions reference
+ * the same global pages, and nothing is copied here: the first of them to append
+ * into the shared, partly filled last page takes a copy of it then (one page of
+ * every layer, on the context stream, all sessions of a microbatch in one
+ * launch; a page of the pool for it).  A page goes back to the pool with its last
+ * holder.  Microbatches whose sessions share their leading pages read those
+ * once for all of them (zr_stage).  The sessions must share one pool; the
+ * child's max_seq_len must hold the parent's window. */
+zr_status zrh_fork(const zrh_backend* parent, zrh_backend* child);
+/* Drops the newest drop_rows rows of the window (rejected drafts) and moves the
+ * position back by as many; pages left empty stay bound to the session.  More
+ * rows than the window holds: ZR_E_INVALID, nothing dropped. */
+zr_status zrh_truncate(zrh_backend* b, int drop_rows);
+/* Pages bound to the session but outside its window (after a trim, a clear or
+ * a truncation) go back to the pool; *released (nullable) is their number. */
+zr_status zrh_release_idle_pages(zrh_backend* b, int* released);
+/* Moves the pages of every session of the pool to the lowest page ids, so that
+ * the free ones are the highest; *moved (nullable) pages are copied, enqueued on
+ * the context stream.  Contents and session-local ids stay.  Microbatches staged
+ * before name the old ids: they, and graphs captured from them, are refused
+ * from then on (ZR_E_INVALID); step graphs and decode pipelines stage every
+ * step and go on.  Page ids that the caller keeps (zrh_block_table) are void. */
+zr_status zrh_pool_compact(zrh_pool* pool, int* moved);
+/* Pages of the pool held by more than one session. */
+int zrh_pool_shared_pages(const zrh_pool* pool);
+
 /* ------------------------------------------------------ fast-path planner --- */
 /* FastPathBackendContext (fast_path.rs:102-108) of one session, as
  * ProviderRuntimeCore::fast_path_context builds it (backend.rs:748-755).  The

@@ -118,6 +118,7 @@ SIGNATURES = [
     ("zr_kv_pool_create", C.c_int, [C.c_void_p, C.c_int]),
     ("zr_kv_pool_pages", C.c_int, [C.c_void_p]),
     ("zr_kv_pool_bytes", C.c_uint64, [C.c_void_p]),
+    ("zr_kv_pool_data", C.c_void_p, [C.c_void_p]),
     ("zr_forward", C.c_int, [C.c_void_p, C.POINTER(Microbatch), c_u32_p, c_f32_p, c_f32_p]),
     ("zr_stage", C.c_int, [C.c_void_p, C.POINTER(Microbatch), c_void_pp]),
     ("zr_staged_destroy", None, [C.c_void_p]),
@@ -148,6 +149,8 @@ SIGNATURES = [
     ("zr_transfer_destroy", None, [C.c_void_p]),
     ("zr_kv_export_cbor", C.c_int, [C.c_void_p, c_int_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_int,
                                     C.c_void_p, C.c_size_t, C.POINTER(C.c_size_t)]),
+    ("zr_kv_copy_pages", C.c_int, [C.c_void_p, c_int_p, c_int_p, C.c_int]),
+    ("zr_kv_copy_pages_async", C.c_int, [C.c_void_p, c_int_p, c_int_p, C.c_int]),
     ("zr_kv_read_pages", C.c_int, [C.c_void_p, C.c_int, c_int_p, C.c_int, C.c_void_p]),
     ("zr_argmax", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     ("zr_argmax_noalloc", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
@@ -197,6 +200,11 @@ SIGNATURES = [
     ("zrh_import_kv_cbor", C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_int]),
     ("zrh_clear", None, [C.c_void_p]),
     ("zrh_release_pages", C.c_int, [C.c_void_p]),
+    ("zrh_fork", C.c_int, [C.c_void_p, C.c_void_p]),
+    ("zrh_truncate", C.c_int, [C.c_void_p, C.c_int]),
+    ("zrh_release_idle_pages", C.c_int, [C.c_void_p, c_int_p]),
+    ("zrh_pool_compact", C.c_int, [C.c_void_p, c_int_p]),
+    ("zrh_pool_shared_pages", C.c_int, [C.c_void_p]),
     ("zrh_get_fast_path_context", C.c_int, [C.c_void_p, C.POINTER(FastPathContext)]),
     ("zrh_fast_path_plan_decode", C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(FastPathPlan)]),
     ("zrh_fast_path_stage_decode", C.c_int, [C.POINTER(FastPathPlan), c_void_pp, C.c_int, c_u32_p, c_u32_p,

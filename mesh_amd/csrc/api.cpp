@@ -318,6 +318,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     if (fixed && stride > fixed->stride) return no_fit("block table stride");
     const int blob_stride = fixed ? fixed->stride : stride;
     st->ctx = ctx;
+    st->page_epoch = ctx->page_epoch;
     st->num_seqs = S;
     st->total_q = total_q;
     st->stride = blob_stride;
@@ -1000,6 +1001,7 @@ zr_status zr_kv_pool_create(zr_context* ctx, int n_pages) {
 }
 
 int zr_kv_pool_pages(const zr_context* ctx) { return ctx ? ctx->n_pages : 0; }
+void* zr_kv_pool_data(const zr_context* ctx) { return ctx ? ctx->kv_pool : nullptr; }
 uint64_t zr_kv_pool_bytes(const zr_context* ctx) {
     return ctx ? (uint64_t)ctx->page_bytes * ctx->n_pages * ctx->desc.num_layers : 0;
 }
@@ -1032,10 +1034,18 @@ void zr_staged_destroy(zr_staged* s) {
     delete st;
 }
 
+// A microbatch staged before a compaction names pages that have moved.
+static zr_status pages_current(zr_context* ctx, uint64_t page_epoch) {
+    if (page_epoch != ctx->page_epoch)
+        return set_err(ctx, ZR_E_INVALID, "staged before the pool's pages were compacted: stage it again");
+    return ZR_OK;
+}
+
 zr_status zr_forward_staged_async(zr_context* ctx, zr_staged* s, const uint32_t* d_tokens, uint32_t* d_out_tokens,
                                   float* d_out_logits) {
     StagedMeta* st = (StagedMeta*)s;
     if (!ctx || !st || st->ctx != ctx) return set_global_err(ZR_E_INVALID, "staged microbatch of another context");
+    if (zr_status rc = pages_current(ctx, st->page_epoch)) return rc;
     return run_forward(ctx, st, d_tokens, d_out_tokens, d_out_logits, nullptr, false);
 }
 
@@ -1064,6 +1074,7 @@ struct zr_graph {
     bool token_check = false;  // the step copies the device id-check word to the host
     uint64_t buffer_epoch = 0; // the context's buffer epoch at capture
     uint64_t staged_id = 0;    // the staged microbatch the graph replays
+    uint64_t page_epoch = 0;   // ... and the page ids it was staged with
 };
 
 zr_status zr_graph_capture_staged(zr_context* ctx, zr_staged* s, const uint32_t* d_tokens, uint32_t* d_out_tokens,
@@ -1071,6 +1082,7 @@ zr_status zr_graph_capture_staged(zr_context* ctx, zr_staged* s, const uint32_t*
     StagedMeta* st = (StagedMeta*)s;
     if (!ctx || !st || !out) return set_global_err(ZR_E_INVALID, "null argument");
     if (st->ctx != ctx) return set_err(ctx, ZR_E_INVALID, "staged microbatch of another context");
+    if (zr_status rc = pages_current(ctx, st->page_epoch)) return rc;
     // HIP events recorded by graph nodes do not time (hipEventElapsedTime
     // reports an invalid handle for them), so timing stays eager-only
     if (ctx->timing.enabled) return set_err(ctx, ZR_E_INVALID, "graph capture with per-class timing on");
@@ -1101,6 +1113,7 @@ zr_status zr_graph_capture_staged(zr_context* ctx, zr_staged* s, const uint32_t*
     g->token_check = d_tokens != nullptr;
     g->buffer_epoch = ctx->buffer_epoch;
     g->staged_id = st->id;
+    g->page_epoch = st->page_epoch;
     *out = g;
     return ZR_OK;
 }
@@ -1113,6 +1126,7 @@ zr_status zr_graph_launch(zr_context* ctx, zr_graph* g) {
                        "graph captured before a workspace, the KV pool or weights were reallocated: capture it again");
     if (std::find(ctx->live_staged.begin(), ctx->live_staged.end(), g->staged_id) == ctx->live_staged.end())
         return set_err(ctx, ZR_E_INVALID, "the graph's staged microbatch was destroyed: stage and capture again");
+    if (zr_status rc = pages_current(ctx, g->page_epoch)) return rc;
     ZR_HIP(ctx, hipGraphLaunch(g->exec, ctx->stream));
     if (g->token_check) ctx->token_check_pending = true;
     return ZR_OK;
@@ -1466,7 +1480,7 @@ zr_status zr_pack(zr_context* ctx, const zr_microbatch* mb, int* cu_q, int* cu_k
 // staged by another context is refused before anything launches.
 static zr_status staged_for(zr_context* ctx, const StagedMeta* st) {
     if (st->ctx != ctx) return set_err(ctx, ZR_E_INVALID, "staged microbatch of another context");
-    return ZR_OK;
+    return pages_current(ctx, st->page_epoch);
 }
 
 zr_status zr_rope_kv_write(zr_context* ctx, zr_staged* s, int layer, const float* d_qkv, float* d_q_out, int rope) {
@@ -1879,6 +1893,38 @@ zr_status zr_kv_export_cbor(zr_context* ctx, const int* block_table, int n_pages
     // KVCacheConfig of the device cache (forward_pass.rs:1791-1796): the model's kv heads and head_dim
     const int cfg[4] = {L, ctx->desc.num_kv_heads, ctx->head_dim, cfg_max_seq_len};
     return launch_kv_cbor(ctx, d_k, d_v, L, n_rows, ctx->kv_cols, base_position, cfg, out, capacity, out_len);
+}
+
+// a page copy's pairs lie in the pool, no page is written twice, and none that is read is written
+static zr_status copy_pages_check(zr_context* ctx, const int* src, const int* dst, int n) {
+    if (n < 0) return set_err(ctx, ZR_E_INVALID, "%d pages to copy", n);
+    if (!ctx->kv_pool) return set_err(ctx, ZR_E_INVALID, "KV pool not created");
+    for (int i = 0; i < n; ++i)
+        if (src[i] < 0 || src[i] >= ctx->n_pages || dst[i] < 0 || dst[i] >= ctx->n_pages)
+            return set_err(ctx, ZR_E_INVARIANT, "page copy %d -> %d outside pool of %d", src[i], dst[i], ctx->n_pages);
+    std::vector<int> d(dst, dst + n), s(src, src + n);
+    std::sort(d.begin(), d.end());
+    std::sort(s.begin(), s.end());
+    for (int i = 1; i < n; ++i)
+        if (d[i] == d[i - 1]) return set_err(ctx, ZR_E_INVALID, "page %d is the target of two copies", d[i]);
+    for (size_t i = 0, j = 0; i < d.size() && j < s.size();) {
+        if (d[i] == s[j]) return set_err(ctx, ZR_E_INVALID, "page %d is both read and written by one copy", d[i]);
+        if (d[i] < s[j]) ++i; else ++j;
+    }
+    return ZR_OK;
+}
+
+zr_status zr_kv_copy_pages_async(zr_context* ctx, const int* src, const int* dst, int n) {
+    if (!ctx || (n > 0 && (!src || !dst))) return set_global_err(ZR_E_INVALID, "null argument");
+    if (zr_status rc = copy_pages_check(ctx, src, dst, n)) return rc;
+    ZR_HIP(ctx, hipSetDevice(ctx->device));
+    return launch_kv_copy_pages(ctx, src, dst, n);
+}
+
+zr_status zr_kv_copy_pages(zr_context* ctx, const int* src, const int* dst, int n) {
+    zr_status rc = zr_kv_copy_pages_async(ctx, src, dst, n);
+    if (!rc) ZR_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    return rc;
 }
 
 zr_status zr_kv_read_pages(zr_context* ctx, int layer, const int* pages, int n_pages, void* dst) {

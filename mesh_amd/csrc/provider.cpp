@@ -17,10 +17,18 @@ using zr::set_global_err;
 struct zrh_pool {
     zr_context* ctx = nullptr;
     std::vector<int> free_list;  // LIFO: pop_back
-    // Global pages popped while a host call is open, in pop order, so that a
-    // failed call can give them back (PoolTxn).
-    std::vector<int> popped;
+    // Sessions that hold each global page (0: free).  More than one after a
+    // fork: such a page is only read; its first writer takes a copy.
+    std::vector<int> refs;
+    // What an open host call has taken, in order, so that a failed call can
+    // give it back (PoolTxn): a popped page g as g, a reference to a shared
+    // page g given up as ~g.
+    std::vector<int> taken;
+    // Page copies (source, target) that the open host call's writes need
+    // first, in order (flush_copies)
+    std::vector<std::pair<int, int>> copies;
     int txn_depth = 0;
+    std::vector<zrh_backend*> sessions;  // in order of creation
 };
 
 namespace {
@@ -62,33 +70,77 @@ namespace {
 // A host call that fails leaves the pool as it found it.  Sessions restore
 // their saved page tables on failure, and the global pages that were bound to
 // them during the call go back onto the free list in reverse pop order, which
-// restores the LIFO order exactly.  Calls nest (a chunked prefill runs one
-// microbatch per chunk): each rolls back only what was popped after its mark.
+// restores the LIFO order exactly (references to shared pages given up
+// during the call come back in the same order).  Calls nest (a chunked prefill
+// runs one microbatch per chunk): each rolls back only what was taken after
+// its mark.
 class PoolTxn {
   public:
-    explicit PoolTxn(zrh_pool* pool) : pool_(pool), mark_(pool ? pool->popped.size() : 0) {
+    explicit PoolTxn(zrh_pool* pool)
+        : pool_(pool), mark_(pool ? pool->taken.size() : 0), copies_(pool ? pool->copies.size() : 0) {
         if (pool_) ++pool_->txn_depth;
     }
     ~PoolTxn() {
-        if (pool_ && --pool_->txn_depth == 0) pool_->popped.clear();
+        if (pool_ && --pool_->txn_depth == 0) {
+            pool_->taken.clear();
+            pool_->copies.clear();
+        }
     }
     PoolTxn(const PoolTxn&) = delete;
     PoolTxn& operator=(const PoolTxn&) = delete;
     void rollback() {
         if (!pool_) return;
-        while (pool_->popped.size() > mark_) {
-            pool_->free_list.push_back(pool_->popped.back());
-            pool_->popped.pop_back();
+        while (pool_->taken.size() > mark_) {
+            const int g = pool_->taken.back();
+            pool_->taken.pop_back();
+            if (g >= 0) {
+                pool_->refs[g] = 0;
+                pool_->free_list.push_back(g);
+            } else {
+                ++pool_->refs[~g];
+            }
         }
+        if (pool_->copies.size() > copies_) pool_->copies.resize(copies_);  // (fewer: they have run)
     }
 
   private:
     zrh_pool* pool_;
-    size_t mark_;
+    size_t mark_, copies_;
 };
 
 zr_status fail(zrh_backend* b, zr_status code, const char* msg, int a = 0, int c = 0, int d = 0) {
     return set_err(b ? b->ctx : nullptr, code, msg, a, c, d);
+}
+
+// A fresh global page for local page `local`: from the pool, or, where that is
+// empty, from another idle local page of the session.
+zr_status bind_global(zrh_backend* b, int local, int* out) {
+    zrh_pool* pool = b->pool;
+    if (!pool) return fail(b, ZR_E_INVALID, "the session's KV pool was destroyed");
+    if (!pool->free_list.empty()) {
+        *out = pool->free_list.back();
+        pool->free_list.pop_back();
+        pool->refs[*out] = 1;
+        if (pool->txn_depth) pool->taken.push_back(*out);
+        return ZR_OK;
+    }
+    for (auto it = b->kv.free_pages.rbegin(); it != b->kv.free_pages.rend(); ++it)
+        if (b->kv.pages[*it].global >= 0) {
+            *out = b->kv.pages[*it].global;
+            b->kv.pages[*it].global = -1;
+            return ZR_OK;
+        }
+    return fail(b, ZR_E_OOM, "KV pool exhausted: no free global page for local page %d", local);
+}
+
+// A local page that leaves the window keeps its global page for reuse, unless
+// other sessions hold that page too: then the reference goes.
+void drop_shared(zrh_backend* b, PageEntry& p) {
+    zrh_pool* pool = b->pool;
+    if (!pool || p.global < 0 || pool->refs[p.global] <= 1) return;
+    --pool->refs[p.global];
+    if (pool->txn_depth) pool->taken.push_back(~p.global);
+    p.global = -1;
 }
 
 // allocate_page (forward_pass.rs:396-424): LIFO reuse, else a new local page
@@ -100,17 +152,15 @@ zr_status allocate_page(zrh_backend* b, int* out) {
         kv.free_pages.pop_back();
         if (kv.pages[idx].active)
             return fail(b, ZR_E_INVARIANT, "Device KV allocator attempted to reuse page %d while it was Active", idx);
+        if (kv.pages[idx].global < 0)  // it gave up a shared page
+            if (zr_status rc = bind_global(b, idx, &kv.pages[idx].global)) return rc;
         kv.pages[idx].used_rows = 0;
         kv.pages[idx].active = true;
         *out = idx;
         return ZR_OK;
     }
-    if (b->pool->free_list.empty())
-        return fail(b, ZR_E_OOM, "KV pool exhausted: no free global page for local page %d", (int)kv.pages.size());
     PageEntry pe;
-    pe.global = b->pool->free_list.back();
-    b->pool->free_list.pop_back();
-    if (b->pool->txn_depth) b->pool->popped.push_back(pe.global);
+    if (zr_status rc = bind_global(b, (int)kv.pages.size(), &pe.global)) return rc;
     pe.active = true;
     kv.pages.push_back(pe);
     *out = (int)kv.pages.size() - 1;
@@ -124,8 +174,47 @@ zr_status release_page(zrh_backend* b, int idx) {
     if (!kv.pages[idx].active) return fail(b, ZR_E_INVARIANT, "Device KV allocator double-freed page %d", idx);
     kv.pages[idx].used_rows = 0;
     kv.pages[idx].active = false;
+    drop_shared(b, kv.pages[idx]);
     kv.free_pages.push_back(idx);
     return ZR_OK;
+}
+
+// A shared page about to be written: the session takes a copy, unless it is the
+// page's last holder.
+zr_status own_page(zrh_backend* b, int idx) {
+    const int shared = b->kv.pages[idx].global;
+    if (!b->pool || b->pool->refs[shared] <= 1) return ZR_OK;
+    int own = -1;
+    if (zr_status rc = bind_global(b, idx, &own)) return rc;
+    drop_shared(b, b->kv.pages[idx]);
+    b->kv.pages[idx].global = own;
+    b->pool->copies.push_back({shared, own});
+    return ZR_OK;
+}
+
+// Enqueues the copies that the open host call's writes need, before its
+// launches (the same stream).  They run in order: a copy that reads or writes a
+// page of those before it starts another launch.
+zr_status flush_copies(zrh_pool* pool) {
+    if (!pool || pool->copies.empty()) return ZR_OK;
+    std::vector<std::pair<int, int>> todo;
+    todo.swap(pool->copies);
+    if (!pool->ctx) return ZR_OK;  // bookkeeping only: no page has contents
+    std::vector<int> src, dst;
+    auto send = [&]() {
+        const zr_status rc = zr_kv_copy_pages_async(pool->ctx, src.data(), dst.data(), (int)src.size());
+        src.clear();
+        dst.clear();
+        return rc;
+    };
+    for (const auto& c : todo) {
+        auto in = [&](const std::vector<int>& v, int g) { return std::find(v.begin(), v.end(), g) != v.end(); };
+        if (in(dst, c.first) || in(dst, c.second) || in(src, c.second))
+            if (zr_status rc = send()) return rc;
+        src.push_back(c.first);
+        dst.push_back(c.second);
+    }
+    return send();
 }
 
 // reclaim_unused_pages (448-460)
@@ -142,10 +231,12 @@ zr_status reclaim_unused(zrh_backend* b) {
 }
 
 // DeviceLayerKVCache::clear (840-850): free list re-seeded 0..n
-void clear_kv(SessionKV& kv) {
+void clear_kv(zrh_backend* b) {
+    SessionKV& kv = b->kv;
     for (PageEntry& p : kv.pages) {
         p.used_rows = 0;
         p.active = false;
+        drop_shared(b, p);
     }
     kv.free_pages.clear();
     for (int p = 0; p < (int)kv.pages.size(); ++p) kv.free_pages.push_back(p);
@@ -162,7 +253,7 @@ zr_status retain_suffix(zrh_backend* b, int keep) {
     if (seq <= keep) return ZR_OK;
     if (keep == 0) {
         const int base = kv.base_position;
-        clear_kv(kv);
+        clear_kv(b);
         kv.base_position = base + seq;
         return ZR_OK;
     }
@@ -190,6 +281,7 @@ zr_status retain_suffix(zrh_backend* b, int keep) {
 // ensure_writable_tail (353-394) + the row bookkeeping of append (462-521)
 zr_status reserve_rows(zrh_backend* b, int rows) {
     SessionKV& kv = b->kv;
+    if (!b->pool) return fail(b, ZR_E_INVALID, "the session's KV pool was destroyed");
     int done = 0;
     while (done < rows) {
         int idx;
@@ -205,6 +297,8 @@ zr_status reserve_rows(zrh_backend* b, int rows) {
                             tail.page_index, tail.start_row + tail.row_count, tp.used_rows);
             if (kPageRows - tp.used_rows > 0) {
                 idx = tail.page_index;
+                zr_status rc = own_page(b, idx);
+                if (rc) return rc;
             } else {
                 zr_status rc = allocate_page(b, &idx);
                 if (rc) return rc;
@@ -231,6 +325,15 @@ zr_status append_rows(zrh_backend* b, int rows) {
         if (rc) return rc;
     }
     return reserve_rows(b, rows);
+}
+
+// One holder fewer of global page g; the last one's goes back onto the free list.
+void free_global(zrh_pool* pool, int g) {
+    if (pool && g >= 0 && --pool->refs[g] == 0) pool->free_list.push_back(g);
+}
+
+int bound_pages(const SessionKV& kv) {
+    return (int)std::count_if(kv.pages.begin(), kv.pages.end(), [](const PageEntry& p) { return p.global >= 0; });
 }
 
 // Canonical device table of the live window: global pages oldest first,
@@ -331,6 +434,11 @@ zr_status assemble(zrh_backend* const* backends, int n, const int* q_len, bool d
         saved.restore(backends, n, txn);
         return rc;
     }
+    rc = flush_copies(backends[0]->pool);
+    if (rc) {
+        saved.restore(backends, n, txn);
+        return rc;
+    }
     out.tables.assign((size_t)n * out.stride, 0);
     for (int i = 0; i < n; ++i) std::copy(tables[i].begin(), tables[i].end(), out.tables.begin() + (size_t)i * out.stride);
     return ZR_OK;
@@ -382,6 +490,7 @@ zr_status zrh_pool_create(zr_context* ctx, const int* initial_order, int n, zrh_
     if (pages <= 0) return set_err(ctx, ZR_E_INVALID, ctx ? "KV pool not created" : "pool of %d pages", n);
     zrh_pool* p = new zrh_pool();
     p->ctx = ctx;
+    p->refs.assign(pages, 0);
     if (initial_order) {
         if (n != pages) {
             delete p;
@@ -403,7 +512,11 @@ zr_status zrh_pool_create(zr_context* ctx, const int* initial_order, int n, zrh_
     return ZR_OK;
 }
 
-void zrh_pool_destroy(zrh_pool* pool) { delete pool; }
+void zrh_pool_destroy(zrh_pool* pool) {
+    if (!pool) return;
+    for (zrh_backend* b : pool->sessions) b->pool = nullptr;  // its sessions hold no page any more
+    delete pool;
+}
 int zrh_pool_free_pages(const zrh_pool* pool) { return pool ? (int)pool->free_list.size() : 0; }
 
 zr_status zrh_backend_create(zrh_pool* pool, int max_seq_len, zrh_backend** out) {
@@ -412,6 +525,7 @@ zr_status zrh_backend_create(zrh_pool* pool, int max_seq_len, zrh_backend** out)
     b->pool = pool;
     b->ctx = pool->ctx;
     b->max_seq_len = max_seq_len;
+    pool->sessions.push_back(b);
     *out = b;
     return ZR_OK;
 }
@@ -419,6 +533,10 @@ zr_status zrh_backend_create(zrh_pool* pool, int max_seq_len, zrh_backend** out)
 void zrh_backend_destroy(zrh_backend* b) {
     if (!b) return;
     zrh_release_pages(b);
+    if (b->pool) {
+        auto& live = b->pool->sessions;
+        live.erase(std::find(live.begin(), live.end(), b));
+    }
     delete b;
 }
 
@@ -429,7 +547,7 @@ zr_status zrh_prefill(zrh_backend* b, const uint32_t* tokens, int n, float* logi
     const SessionKV saved = b->kv;
     const int saved_pos = b->position;
     // clear_cache + keep the last window (forward_pass.rs:2101-2105)
-    clear_kv(b->kv);
+    clear_kv(b);
     b->position = 0;
     const int window = std::max(b->max_seq_len, 1);
     const int start = n > window ? n - window : 0;
@@ -518,7 +636,7 @@ int zrh_cache_seq_len(const zrh_backend* b) { return b ? b->kv.seq_len : 0; }
 int zrh_sequence_position(const zrh_backend* b) { return b ? b->position : 0; }
 int zrh_logical_kv_tokens(const zrh_backend* b) { return b ? b->position - b->kv.base_position : 0; }
 int zrh_base_position(const zrh_backend* b) { return b ? b->kv.base_position : 0; }
-int zrh_allocated_pages(const zrh_backend* b) { return b ? (int)b->kv.pages.size() : 0; }
+int zrh_allocated_pages(const zrh_backend* b) { return b ? bound_pages(b->kv) : 0; }
 
 uint64_t zrh_live_kv_cache_bytes(const zrh_backend* b) {
     // DeviceLayerKVCache::memory_usage (883-891) summed over layers, at the
@@ -526,7 +644,7 @@ uint64_t zrh_live_kv_cache_bytes(const zrh_backend* b) {
     if (!b || !b->ctx) return 0;
     const zr_context* ctx = b->ctx;
     const uint64_t esz = ctx->desc.kv_dtype == ZR_DTYPE_BF16 ? 2 : 4;
-    return (uint64_t)b->kv.pages.size() * kPageRows * ctx->kv_cols * esz * 2 * ctx->desc.num_layers;
+    return (uint64_t)bound_pages(b->kv) * kPageRows * ctx->kv_cols * esz * 2 * ctx->desc.num_layers;
 }
 
 int zrh_block_table(const zrh_backend* b, uint32_t* page_ids, int* start_tokens, int* token_counts, int* global_pages,
@@ -611,7 +729,7 @@ static zr_status import_rows(zrh_backend* b, int rows, int base_position, int ne
     PoolTxn txn(b->pool);
     const SessionKV saved = b->kv;
     const int saved_pos = b->position;
-    clear_kv(b->kv);
+    clear_kv(b);
     b->kv.base_position = base_position;
     zr_status rc = ZR_OK;
     if (rows > 0) {
@@ -745,16 +863,125 @@ zr_status zrh_import_kv_cbor(zrh_backend* b, const uint8_t* bytes, size_t len, i
 
 void zrh_clear(zrh_backend* b) {
     if (!b) return;
-    clear_kv(b->kv);
+    clear_kv(b);
     b->position = 0;
 }
 
 zr_status zrh_release_pages(zrh_backend* b) {
     if (!b) return set_global_err(ZR_E_INVALID, "null backend");
-    for (const PageEntry& p : b->kv.pages)
-        if (p.global >= 0) b->pool->free_list.push_back(p.global);
+    for (const PageEntry& p : b->kv.pages) free_global(b->pool, p.global);
     b->kv = SessionKV();
     b->position = 0;
+    return ZR_OK;
+}
+
+zr_status zrh_fork(const zrh_backend* parent, zrh_backend* child) {
+    if (!parent || !child) return set_global_err(ZR_E_INVALID, "null backend");
+    if (parent == child) return set_err(child->ctx, ZR_E_INVALID, "a session cannot be forked into itself");
+    if (!child->pool || parent->pool != child->pool)
+        return set_err(child->ctx, ZR_E_INVALID, "fork between KV pools");
+    const SessionKV& from = parent->kv;
+    if (from.base_position + from.seq_len != parent->position)
+        return set_err(child->ctx, ZR_E_INVARIANT, "Forward pass position %d diverged from KV cache next position %d",
+                       parent->position, from.base_position + from.seq_len);
+    if (from.seq_len > std::max(child->max_seq_len, 1))
+        return set_err(child->ctx, ZR_E_INVALID, "fork of %d rows into a %d-token window", from.seq_len,
+                       child->max_seq_len);
+    SessionKV kv;
+    for (const Span& s : from.spans) {
+        kv.spans.push_back({(int)kv.pages.size(), s.start_row, s.row_count});
+        kv.pages.push_back(from.pages[s.page_index]);
+        ++child->pool->refs[kv.pages.back().global];
+    }
+    kv.seq_len = from.seq_len;
+    kv.base_position = from.base_position;
+    zrh_release_pages(child);
+    child->kv = std::move(kv);
+    child->position = parent->position;
+    return ZR_OK;
+}
+
+zr_status zrh_truncate(zrh_backend* b, int drop_rows) {
+    if (!b) return set_global_err(ZR_E_INVALID, "null backend");
+    SessionKV& kv = b->kv;
+    if (drop_rows < 0 || drop_rows > kv.seq_len)
+        return set_err(b->ctx, ZR_E_INVALID, "truncation by %d of %d cached rows", drop_rows, kv.seq_len);
+    PoolTxn txn(b->pool);
+    const SessionKV saved = kv;
+    for (int drop = drop_rows; drop > 0;) {
+        Span& back = kv.spans.back();
+        PageEntry& pg = kv.pages[back.page_index];
+        if (drop < back.row_count) {
+            back.row_count -= drop;
+            pg.used_rows -= drop;
+            drop = 0;
+            continue;
+        }
+        drop -= back.row_count;
+        const int idx = back.page_index;
+        kv.spans.pop_back();
+        if (zr_status rc = release_page(b, idx)) {
+            kv = saved;
+            txn.rollback();
+            return rc;
+        }
+    }
+    kv.seq_len -= drop_rows;
+    b->position -= drop_rows;
+    return ZR_OK;
+}
+
+zr_status zrh_release_idle_pages(zrh_backend* b, int* released) {
+    if (!b) return set_global_err(ZR_E_INVALID, "null backend");
+    SessionKV& kv = b->kv;
+    int n = 0;
+    for (const int idx : kv.free_pages)
+        if (kv.pages[idx].global >= 0) {
+            free_global(b->pool, kv.pages[idx].global);
+            kv.pages[idx].global = -1;
+            ++n;
+        }
+    if (released) *released = n;
+    return ZR_OK;
+}
+
+int zrh_pool_shared_pages(const zrh_pool* pool) {
+    return pool ? (int)std::count_if(pool->refs.begin(), pool->refs.end(), [](int r) { return r > 1; }) : 0;
+}
+
+zr_status zrh_pool_compact(zrh_pool* pool, int* moved) {
+    if (!pool) return set_global_err(ZR_E_INVALID, "null pool");
+    const int n = (int)pool->refs.size();
+    const int used = n - (int)std::count(pool->refs.begin(), pool->refs.end(), 0);
+    // pages of a window have contents to move; idle ones are only bound elsewhere
+    std::vector<char> live(n, 0);
+    for (const zrh_backend* b : pool->sessions)
+        for (const Span& s : b->kv.spans) live[b->kv.pages[s.page_index].global] = 1;
+    std::vector<int> to(n), src, dst;
+    int hole = 0;
+    for (int g = 0; g < n; ++g) {
+        to[g] = g;
+        if (g < used || pool->refs[g] == 0) continue;
+        while (pool->refs[hole] != 0) ++hole;
+        to[g] = hole++;
+        if (live[g]) {
+            src.push_back(g);
+            dst.push_back(to[g]);
+        }
+    }
+    if (moved) *moved = (int)src.size();
+    if (pool->ctx && !src.empty())
+        if (zr_status rc = zr_kv_copy_pages_async(pool->ctx, src.data(), dst.data(), (int)src.size())) return rc;
+    for (zrh_backend* b : pool->sessions)
+        for (PageEntry& p : b->kv.pages)
+            if (p.global >= 0) p.global = to[p.global];
+    std::vector<int> refs(n, 0);
+    for (int g = 0; g < n; ++g)
+        if (pool->refs[g]) refs[to[g]] = pool->refs[g];
+    pool->refs.swap(refs);
+    pool->free_list.clear();
+    for (int g = n - 1; g >= used; --g) pool->free_list.push_back(g);
+    if (pool->ctx) ++pool->ctx->page_epoch;
     return ZR_OK;
 }
 
@@ -1106,6 +1333,7 @@ zr_status zrh_kv_reserve(zrh_backend* b, int rows) {
     PoolTxn txn(b->pool);
     const SessionKV saved = b->kv;
     zr_status rc = append_rows(b, rows);
+    if (!rc) rc = flush_copies(b->pool);
     if (rc) {
         b->kv = saved;
         txn.rollback();
@@ -1117,10 +1345,12 @@ zr_status zrh_kv_reserve(zrh_backend* b, int rows) {
 
 zr_status zrh_retain_suffix(zrh_backend* b, int keep_rows) {
     if (!b) return set_global_err(ZR_E_INVALID, "null backend");
+    PoolTxn txn(b->pool);
     const SessionKV saved = b->kv;
     zr_status rc = retain_suffix(b, keep_rows);
     if (rc) {
         b->kv = saved;
+        txn.rollback();
         return rc;
     }
     b->position = b->kv.base_position + b->kv.seq_len;

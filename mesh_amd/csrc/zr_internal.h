@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <string>
 #include <vector>
 
@@ -223,6 +224,9 @@ struct zr_context {
     // workspace regrown, the KV pool or weights replaced): graphs captured
     // before hold its old address and are refused at launch
     uint64_t buffer_epoch = 0;
+    // bumped when live pages move to other page ids (zrh_pool_compact): staged
+    // microbatches hold the old ids and are refused
+    uint64_t page_epoch = 0;
     // staged microbatches (zr_stage) not yet destroyed: a graph replays its
     // staged blob, so it is refused once that blob is gone
     std::vector<uint64_t> live_staged;
@@ -301,6 +305,7 @@ PlainAttnPlan plain_attention_plan(int head_dim, int kv_heads, int G, const int*
 struct StagedMeta {
     zr_context* ctx = nullptr;
     uint64_t id = 0;          // zr_stage handle id (zr_context::live_staged)
+    uint64_t page_epoch = 0;  // zr_context::page_epoch when staged
     int num_seqs = 0, total_q = 0, stride = 0;
     int max_kv = 0;           // max kv_after over sequences
     int n_attn_items = 0;     // attention work items (per kv head)
@@ -422,6 +427,9 @@ zr_status launch_attention_rope(zr_context* ctx, StagedMeta* st, int layer, cons
 zr_status launch_kv_copy(zr_context* ctx, int layer_begin, int layer_end, const int* d_table,
                          int first_offset, int first_row, int n_rows, float* k, float* v,
                          int to_pool);
+// pool[l][dst[i]] = pool[l][src[i]] in every layer (host arrays, free on return);
+// the caller has checked them: in the pool, dst distinct and none among src.
+zr_status launch_kv_copy_pages(zr_context* ctx, const int* src, const int* dst, int n);
 zr_status launch_argmax(zr_context* ctx, const float* x, int rows, int cols, uint32_t* out);
 // The same with the partials in the library's fixed device array (no
 // allocation; rows x ceil(cols / 4096) <= kNoAllocArgmaxPairs).

@@ -401,6 +401,24 @@ class DeviceContext:
     def kv_pool_bytes(self) -> int:
         return int(self.lib.zr_kv_pool_bytes(self.h))
 
+    @property
+    def shared_pages(self) -> int:
+        """Pool pages held by more than one session (zrh_pool_shared_pages)."""
+        return self.lib.zrh_pool_shared_pages(self.pool)
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int]):
+        """Page dst[i] becomes a copy of page src[i] in every layer (zr_kv_copy_pages)."""
+        a, b = (np.ascontiguousarray(x, np.int32) for x in (src, dst))
+        if a.shape != b.shape or a.ndim != 1:
+            raise ValueError(f"page copies of shapes {a.shape} -> {b.shape}")
+        self.check(self.lib.zr_kv_copy_pages(self.h, _ptr(a, C.c_int), _ptr(b, C.c_int), a.size))
+
+    def compact_pages(self) -> int:
+        """Moves every session's pages to the lowest page ids (zrh_pool_compact); the pages copied."""
+        moved = C.c_int()
+        self.check(self.lib.zrh_pool_compact(self.pool, C.byref(moved)))
+        return moved.value
+
     def kv_head_map(self) -> List[int]:
         n = C.c_int()
         out = np.zeros(max(self.geo.num_heads, 1), np.uint32)
@@ -659,6 +677,24 @@ class RocmExecutionBackend:
 
     def release_pages(self):
         self.ctx.check(self.lib.zrh_release_pages(self.h))
+
+    # -- shared and spare pages ------------------------------------------------------------
+    def fork(self, max_seq_len: Optional[int] = None) -> "RocmExecutionBackend":
+        """A second session with this one's window and position, on the same pages
+        until either writes into a shared one (zrh_fork)."""
+        child = self.ctx.new_backend(self.max_seq_len if max_seq_len is None else max_seq_len)
+        self.ctx.check(self.lib.zrh_fork(self.h, child.h))
+        return child
+
+    def truncate(self, drop_rows: int):
+        """Drops the newest rows of the window and moves the position back (zrh_truncate)."""
+        self.ctx.check(self.lib.zrh_truncate(self.h, int(drop_rows)))
+
+    def release_idle_pages(self) -> int:
+        """Returns the session's pages outside its window to the pool (zrh_release_idle_pages)."""
+        n = C.c_int()
+        self.ctx.check(self.lib.zrh_release_idle_pages(self.h, C.byref(n)))
+        return n.value
 
     # -- page-table introspection --------------------------------------------------------
     def block_table(self):
