@@ -162,6 +162,23 @@ zr_status zr_forward(zr_context* ctx, const zr_microbatch* mb, uint32_t* out_tok
  * microbatch of another context") for one staged by another context. */
 typedef struct zr_staged zr_staged;
 zr_status zr_stage(zr_context* ctx, const zr_microbatch* mb, zr_staged** out);
+/* Sequences of one staged microbatch whose block tables name the same leading
+ * pages (forked sessions, zrh_fork; a common system prompt) share them: the
+ * attention stage reads each shared run once for the query rows of all its
+ * holders, the rest of every window by itself, and joins the two.  zr_stage
+ * finds the runs (shared at any depth: a batch may hold several prompts, and a
+ * prompt's forks forks of their own).  Runs of fewer than 4 pages, sequences with
+ * prefill-chunk rows and plain-layout pools are not shared; neither is anything
+ * with ZR_SHARED_PREFIX=0 in the environment.  The values are those of
+ * separate reads within the rounding of f32 sums.  No reference counterpart. */
+typedef struct {
+    int segments;     /* shared runs of pages */
+    int sequences;    /* sequences that read through them */
+    int rows;         /* ... and their query rows */
+    int units;        /* work units of the shared launch, per kv head */
+    int pages_saved;  /* page reads saved per layer and kv head: sum of (holders - 1) x pages */
+} zr_prefix_info;
+zr_status zr_staged_prefix_info(const zr_staged* st, zr_prefix_info* out);
 void zr_staged_destroy(zr_staged* st);
 /* Enqueues the forward pass on the context stream without synchronising.
  * d_tokens: device [sum q_len] input ids, or NULL to use the staged ids.
@@ -247,6 +264,8 @@ zr_status zr_rope_kv_write(zr_context* ctx, zr_staged* st, int layer, const floa
  * staged microbatch for `layer`: d_q device [sum q_len, q_cols] f32 (RoPE'd),
  * d_out device [sum q_len, q_cols] f32. */
 zr_status zr_attention(zr_context* ctx, zr_staged* st, int layer, const float* d_q, float* d_out);
+/* zr_attention enqueued on the context stream without waiting. */
+zr_status zr_attention_async(zr_context* ctx, zr_staged* st, int layer, const float* d_q, float* d_out);
 /* Diagnostic, no counterpart in the reference: the HBM rate the decode
  * attention launch's access pattern can reach.  Launches `repeats` times
  * (1..10000) a read-only copy of that launch's page stream for the staged

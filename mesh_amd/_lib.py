@@ -68,6 +68,11 @@ class StepGraphStats(C.Structure):
                 ("metadata_bytes", C.c_size_t)]
 
 
+class PrefixInfo(C.Structure):
+    _fields_ = [("segments", C.c_int), ("sequences", C.c_int), ("rows", C.c_int), ("units", C.c_int),
+                ("pages_saved", C.c_int)]
+
+
 class ExecutorContract(C.Structure):
     _fields_ = [("executor_class", C.c_char_p), ("optimization_profile", C.c_char_p),
                 ("n_host_kernels", C.c_int), ("host_kernels", C.POINTER(C.c_char_p)),
@@ -121,6 +126,7 @@ SIGNATURES = [
     ("zr_kv_pool_data", C.c_void_p, [C.c_void_p]),
     ("zr_forward", C.c_int, [C.c_void_p, C.POINTER(Microbatch), c_u32_p, c_f32_p, c_f32_p]),
     ("zr_stage", C.c_int, [C.c_void_p, C.POINTER(Microbatch), c_void_pp]),
+    ("zr_staged_prefix_info", C.c_int, [C.c_void_p, C.POINTER(PrefixInfo)]),
     ("zr_staged_destroy", None, [C.c_void_p]),
     ("zr_forward_staged_async", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     ("zr_synchronize", C.c_int, [C.c_void_p]),
@@ -136,6 +142,7 @@ SIGNATURES = [
     ("zr_pack", C.c_int, [C.c_void_p, C.POINTER(Microbatch), c_int_p, c_int_p, c_int_p, c_int_p, c_int_p]),
     ("zr_rope_kv_write", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int]),
     ("zr_attention", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
+    ("zr_attention_async", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
     ("zr_kv_read_probe", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_double)]),
     ("zr_rope_attention", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int]),
     ("zr_kv_gather", C.c_int, [C.c_void_p, c_int_p, C.c_int, C.c_int, C.c_int, C.c_int, c_f32_p, c_f32_p]),

@@ -153,11 +153,18 @@ static inline size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
 // Offsets of one staged blob: the host-written inputs and records first, then
 // the arrays the pack stage derives on the device.
 struct BlobLayout {
-    size_t o_qlen, o_kvb, o_fpos, o_foff, o_bt, o_tok, o_arec, o_mrec, o_pblk, o_psplit, host_bytes;
+    size_t o_qlen, o_kvb, o_fpos, o_foff, o_bt, o_tok, o_arec, o_mrec, o_pblk, o_psplit, o_sunit, o_smrg, o_ssrc, o_srow,
+        host_bytes;
     size_t o_cuq, o_cuk, o_pos, o_slot, o_seq, o_last, o_rcs, total_bytes;
 };
 
-static BlobLayout blob_layout(int S, int stride, int total_q, int n_items, int n_merge, int n_pblocks, int head_dim) {
+// records of the shared-prefix launch and its merge
+struct SharedCounts {
+    int units = 0, merges = 0, sources = 0, rows = 0;
+};
+
+static BlobLayout blob_layout(int S, int stride, int total_q, int n_items, int n_merge, int n_pblocks, int head_dim,
+                              const SharedCounts& sh = SharedCounts()) {
     BlobLayout b;
     size_t off = 0;
     auto take = [&](size_t bytes) {
@@ -175,6 +182,10 @@ static BlobLayout blob_layout(int S, int stride, int total_q, int n_items, int n
     b.o_mrec = take(16 * (size_t)std::max(n_merge, 1));
     b.o_pblk = take(16 * (size_t)std::max(n_pblocks, 1));
     b.o_psplit = take(16 * (size_t)std::max(n_pblocks, 1));
+    b.o_sunit = take(32 * (size_t)sh.units);
+    b.o_smrg = take(16 * (size_t)sh.merges);
+    b.o_ssrc = take(16 * (size_t)sh.sources);
+    b.o_srow = take(4 * (size_t)sh.rows);
     b.host_bytes = off;
     b.o_cuq = take(4 * (S + 1));
     b.o_cuk = take(4 * (S + 1));
@@ -360,11 +371,26 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
             }
         }
     }
-    std::vector<int> tile_pages;
+    // Sequences whose rows run as decode tiles and that share their leading pages
+    // leave those pages to the shared-prefix launch: their own tiles begin at
+    // page cover[s].  ZR_SHARED_PREFIX=0: every sequence reads its whole window.
+    auto as_prefill = [&](int s) {
+        const long ql = mb->q_len[s];
+        return prows && ql >= prows && (!f32_kv || ql * G * (mb->kv_before[s] + ql / 2) >= kPrefillF32Work);
+    };
+    std::vector<SharedSegment> segments;
+    std::vector<int> cover(S, 0);
+    const char* shared_env = getenv("ZR_SHARED_PREFIX");
+    if (qpt > 0 && S > 1 && !fixed && !(shared_env && atoi(shared_env) == 0)) {
+        std::vector<char> takes(S);
+        for (int s = 0; s < S; ++s) takes[s] = !as_prefill(s);
+        shared_segments(mb, takes, &segments, &cover);
+    }
+    std::vector<int> tile_pages;  // pages of each tile past its sequence's cover
     std::vector<int4> pblk;  // prefill blocks {seq, r0, nrows, pages}
     for (int s = 0; s < S && qpt > 0; ++s) {
         const int ql = mb->q_len[s], kb = mb->kv_before[s], fo = mb->first_offset[s];
-        if (prows && ql >= prows && (!f32_kv || (long)ql * G * (kb + ql / 2) >= kPrefillF32Work)) {
+        if (as_prefill(s)) {
             for (int r0 = 0; r0 < ql; r0 += prows) {
                 const int nr = std::min(prows, ql - r0);
                 const int last_visible = kb + r0 + nr - 1;
@@ -378,14 +404,15 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
             const int last_visible = kb + q0 + nq - 1;  // logical index of the tile's last key
             const int pages = (fo + last_visible + 1 + kPageRows - 1) / kPageRows;
             st->h_tiles.push_back(make_int4(s, q0, nq, 0));
-            tile_pages.push_back(pages);
+            tile_pages.push_back(pages - cover[s]);
         }
     }
     const int pps = pages_per_split(tile_pages, ctx->local_kv_heads);
     for (size_t t = 0; t < st->h_tiles.size(); ++t) {
         st->h_tiles[t].w = (int)st->h_items.size();
+        const int first = cover[st->h_tiles[t].x];
         for (int pb = 0; pb < tile_pages[t]; pb += pps)
-            st->h_items.push_back(make_int4((int)t, pb, std::min(tile_pages[t], pb + pps), 0));
+            st->h_items.push_back(make_int4((int)t, first + pb, first + std::min(tile_pages[t], pb + pps), 0));
     }
     const int n_decode_tiles = (int)st->h_tiles.size();
     st->n_attn_items = (int)st->h_items.size();
@@ -438,9 +465,68 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
                                             std::min(rows_per_group, b.z - k * rows_per_group), next_item + k * ns));
         next_item += groups * ns;
     }
-    st->n_part_items = next_item;
     st->h_tiles.push_back(make_int4(0, 0, 0, next_item));  // sentinel
     st->n_tiles = (int)st->h_tiles.size() - 1;
+    // Shared segments: units of up to 128 columns (128 / G rows) and a run of
+    // key tiles each; a unit's 16-column groups have one partial item per split,
+    // after the items above.
+    st->h_sunits.clear();
+    st->h_smerge.clear();
+    st->h_ssrc.clear();
+    st->h_srows.clear();
+    st->n_segments = (int)segments.size();
+    st->shared_seqs = st->shared_saved = 0;
+    std::vector<std::vector<int4>> row_src;  // by query row: partials {first item, parts, first column of its 16}
+    std::vector<int> cu_rows(S + 1, 0);
+    for (int s = 0; s < S; ++s) cu_rows[s + 1] = cu_rows[s] + mb->q_len[s];
+    if (!segments.empty()) {
+        row_src.resize(total_q);
+        const int upr = 128 / G, gpr = 16 / G;  // rows per unit and per 16-column group
+        long unit_tiles = 0;
+        for (const SharedSegment& g : segments) {
+            int rows = 0;
+            for (int s : g.members) rows += mb->q_len[s];
+            unit_tiles += (long)((rows + upr - 1) / upr) * ((g.end - g.begin + 1) / 2);
+        }
+        const int unit_tps = (int)std::max<long>(4, (unit_tiles * ctx->local_kv_heads + slots - 1) / slots);
+        for (const SharedSegment& g : segments) {
+            const int row0 = (int)st->h_srows.size();
+            for (int s : g.members)
+                for (int r = cu_rows[s]; r < cu_rows[s + 1]; ++r) st->h_srows.push_back(r);
+            const int rows = (int)st->h_srows.size() - row0;
+            const int nt = (g.end - g.begin + 1) / 2, ns = (nt + unit_tps - 1) / unit_tps;
+            const int groups = (rows + gpr - 1) / gpr;
+            for (int sp = 0; sp < ns; ++sp)  // the units of a run of tiles side by side: they read the same pages
+                for (int r = 0; r < rows; r += upr) {
+                    const int n = std::min(upr, rows - r);
+                    st->h_sunits.push_back(make_int4(g.seq, row0 + r, n | ns << 16, g.begin));
+                    st->h_sunits.push_back(make_int4((int)((long)sp * nt / ns), (int)((long)(sp + 1) * nt / ns),
+                                                     next_item + (r / gpr) * ns + sp, g.end));
+                }
+            for (int r = 0; r < rows; ++r)
+                row_src[st->h_srows[row0 + r]].push_back(make_int4(next_item + (r / gpr) * ns, ns, (r % gpr) * G, 0));
+            next_item += groups * ns;
+            st->shared_saved += ((int)g.members.size() - 1) * (g.end - g.begin);
+        }
+        // ... and the partials of the rows' own pages
+        for (int t = 0; t < n_decode_tiles; ++t) {
+            const int4 tl = st->h_tiles[t];
+            if (!cover[tl.x]) continue;
+            for (int i = 0; i < tl.z; ++i)
+                row_src[cu_rows[tl.x] + tl.y + i].push_back(make_int4(tl.w, st->h_tiles[t + 1].w - tl.w, i * G, 0));
+        }
+        for (int s = 0; s < S; ++s) {
+            if (!cover[s]) continue;
+            ++st->shared_seqs;
+            for (int r = cu_rows[s]; r < cu_rows[s + 1]; ++r) {
+                st->h_smerge.push_back(make_int4(r, (int)st->h_ssrc.size(), (int)row_src[r].size(), 0));
+                st->h_ssrc.insert(st->h_ssrc.end(), row_src[r].begin(), row_src[r].end());
+            }
+        }
+    }
+    st->n_sunits = (int)st->h_sunits.size() / 2;
+    st->n_smerge = (int)st->h_smerge.size();
+    st->n_part_items = next_item;
     // dispatch order: longest items first, so the short ones fill the tail
     st->h_order.resize(st->n_attn_items);
     for (int i = 0; i < st->n_attn_items; ++i) st->h_order[i] = i;
@@ -450,7 +536,8 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     // tiles whose splits need the merge kernel (every prefill group tile has several)
     st->h_merge.clear();
     for (int t = 0; t < st->n_tiles; ++t)
-        if (t >= n_decode_tiles || st->h_tiles[t + 1].w - st->h_tiles[t].w > 1) st->h_merge.push_back(t);
+        if (t >= n_decode_tiles || (st->h_tiles[t + 1].w - st->h_tiles[t].w > 1 && !cover[st->h_tiles[t].x]))
+            st->h_merge.push_back(t);
     st->n_merge = (int)st->h_merge.size();
     // Per-launch records in the order the kernels read them, so that a
     // workgroup's first page and Q loads wait on one metadata load instead of
@@ -467,7 +554,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
             const int first = tl.w, end = st->h_tiles[it.x + 1].w;
             const int seq = tl.x;
             unsigned meta = (unsigned)item;
-            if (end - first == 1) meta |= kAttnSingle;
+            if (end - first == 1 && !cover[seq]) meta |= kAttnSingle;
             if (item == end - 1) meta |= kAttnLast;
             const int* bt = mb->block_tables + (size_t)seq * stride;
             auto pid = [&](int k) { return it.y + k < it.z ? bt[it.y + k] : 0; };
@@ -511,12 +598,14 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     // ZR_ATTN_FUSE_ROPE=1 / 0 forces either path.
     st->pure_decode = !ctx->plain_kv && S > 0 && st->n_pblocks == 0;
     for (int s = 0; s < S && st->pure_decode; ++s) st->pure_decode = mb->q_len[s] == 1;
-    st->fuse_rope = st->pure_decode && pps >= 48;
-    if (st->pure_decode && !st->fuse_rope) {
+    // Not with shared segments, whose units read the rotated q too.
+    const bool may_fuse = st->pure_decode && st->n_sunits == 0;
+    st->fuse_rope = may_fuse && pps >= 48;
+    if (may_fuse && !st->fuse_rope) {
         const GemmPlan qkv = gemm_plan(total_q, ctx->q_cols + 2 * ctx->kv_cols, ctx->desc.hidden, kEpiStore);
         st->fuse_rope = qkv.few_rows && qkv.splits <= 2;
     }
-    if (const char* env = getenv("ZR_ATTN_FUSE_ROPE")) st->fuse_rope = st->pure_decode && atoi(env) != 0;
+    if (const char* env = getenv("ZR_ATTN_FUSE_ROPE")) st->fuse_rope = may_fuse && atoi(env) != 0;
     st->grid_items = st->n_attn_items;
     st->grid_merge = st->n_merge;
     if (fixed) {
@@ -542,8 +631,13 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     }
 
     // one blob: inputs, derived arrays, attention items
+    SharedCounts sh;
+    sh.units = st->n_sunits;
+    sh.merges = st->n_smerge;
+    sh.sources = (int)st->h_ssrc.size();
+    sh.rows = (int)st->h_srows.size();
     const BlobLayout L = blob_layout(S, blob_stride, total_q, st->grid_items, st->grid_merge, st->n_pblocks,
-                                     ctx->head_dim);
+                                     ctx->head_dim, sh);
     const size_t host_bytes = L.host_bytes, total_bytes = L.total_bytes;
     unsigned char* hb;
     if (fixed) {
@@ -588,7 +682,17 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
         memset(hb + L.o_mrec + 16 * (size_t)st->n_merge, 0, 16 * (size_t)(st->grid_merge - st->n_merge));
     if (st->n_pblocks) memcpy(hb + L.o_pblk, st->h_pblocks.data(), 16 * (size_t)st->n_pblocks);
     if (st->n_pblocks) memcpy(hb + L.o_psplit, st->h_psplits.data(), 16 * (size_t)st->n_pblocks);
+    if (st->n_sunits) {
+        memcpy(hb + L.o_sunit, st->h_sunits.data(), 16 * st->h_sunits.size());
+        memcpy(hb + L.o_smrg, st->h_smerge.data(), 16 * st->h_smerge.size());
+        memcpy(hb + L.o_ssrc, st->h_ssrc.data(), 16 * st->h_ssrc.size());
+        memcpy(hb + L.o_srow, st->h_srows.data(), 4 * st->h_srows.size());
+    }
     unsigned char* db = (unsigned char*)st->dev;
+    st->sunits = (int4*)(db + L.o_sunit);
+    st->smerge = (int4*)(db + L.o_smrg);
+    st->ssrc = (int4*)(db + L.o_ssrc);
+    st->srows = (int*)(db + L.o_srow);
     st->q_len = (int*)(db + L.o_qlen);
     st->kv_before = (int*)(db + L.o_kvb);
     st->first_pos = (int*)(db + L.o_fpos);
@@ -1019,6 +1123,17 @@ zr_status zr_stage(zr_context* ctx, const zr_microbatch* mb, zr_staged** out) {
     st->id = ctx->next_staged_id++;
     ctx->live_staged.push_back(st->id);
     *out = (zr_staged*)st;
+    return ZR_OK;
+}
+
+zr_status zr_staged_prefix_info(const zr_staged* s, zr_prefix_info* out) {
+    const StagedMeta* st = (const StagedMeta*)s;
+    if (!st || !out) return set_global_err(ZR_E_INVALID, "null argument");
+    out->segments = st->n_segments;
+    out->sequences = st->shared_seqs;
+    out->rows = st->n_smerge;
+    out->units = st->n_sunits;
+    out->pages_saved = st->shared_saved;
     return ZR_OK;
 }
 
@@ -1503,12 +1618,17 @@ zr_status zr_rope_attention(zr_context* ctx, zr_staged* s, int layer, const floa
     return rc;
 }
 
-zr_status zr_attention(zr_context* ctx, zr_staged* s, int layer, const float* d_q, float* d_out) {
+zr_status zr_attention_async(zr_context* ctx, zr_staged* s, int layer, const float* d_q, float* d_out) {
     StagedMeta* st = (StagedMeta*)s;
     if (!ctx || !st || !d_q || !d_out) return set_global_err(ZR_E_INVALID, "null argument");
     if (zr_status rc = staged_for(ctx, st)) return rc;
     if (layer < 0 || layer >= ctx->desc.num_layers) return set_err(ctx, ZR_E_INVALID, "Invalid layer index: %d", layer);
-    zr_status rc = launch_attention(ctx, st, layer, d_q, d_out, nullptr);
+    ZR_HIP(ctx, hipSetDevice(ctx->device));
+    return launch_attention(ctx, st, layer, d_q, d_out, nullptr);
+}
+
+zr_status zr_attention(zr_context* ctx, zr_staged* s, int layer, const float* d_q, float* d_out) {
+    zr_status rc = zr_attention_async(ctx, s, layer, d_q, d_out);
     if (!rc) ZR_HIP(ctx, hipStreamSynchronize(ctx->stream));
     return rc;
 }

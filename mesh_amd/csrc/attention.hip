@@ -29,6 +29,7 @@
 // Precision: Q and P enter the MFMA as bf16 hi + lo pairs (x = hi + lo to
 // 2^-16), K/V are exact in bf16 pools; f32 pools also split K/V into hi + lo
 // (three products per MFMA pair).  Accumulation is f32 throughout.
+#include "attn_tile.h"
 #include "zr_internal.h"
 
 namespace zr {
@@ -79,23 +80,6 @@ template <int D> struct PageRegs<float, D> {
         }
     }
 };
-
-// x[0..7] as bf16 hi + lo fragments, two values per v_cvt_pk_bf16_f32 (the
-// same bits as split_bf16)
-__device__ inline void split_bf16x8(const float* x, bf16x8& hi, bf16x8& lo) {
-    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
-    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const f32x2 v = {x[2 * j], x[2 * j + 1]};
-        const bf16x2 h = __builtin_convertvector(v, bf16x2);
-        const bf16x2 l = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), bf16x2);
-        hi[2 * j] = h[0];
-        hi[2 * j + 1] = h[1];
-        lo[2 * j] = l[0];
-        lo[2 * j + 1] = l[1];
-    }
-}
 
 __device__ inline bf16x4 to_bf16x4(const float* x, bool lo_part) {
     bf16x4 r;
@@ -596,18 +580,6 @@ struct PrefillArgs {
     size_t out_lo_offset;
 };
 
-typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
-
-__device__ inline float pair_max(float x) {
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-__device__ inline float pair_sum(float x) {
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // Q^T fragments (B operand) of a column: lane holds Q[col][16 ks + 8 h + j]
 // log2(e) / sqrt(d) as hi + lo (scores come out in log2 units).
 template <int D>
@@ -626,51 +598,6 @@ __device__ __forceinline__ void prefill_load_q(const PrefillArgs& a, size_t at, 
         }
         qh[ks] = to_bf16x8(x, false);
         ql[ks] = to_bf16x8(x, true);
-    }
-}
-
-// Scores of keys a column does not see: element i is logical key jbase + 8 (i / 4) + i % 4.
-__device__ __forceinline__ void prefill_mask(f32x16& s, int jbase, int jmax) {
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int j = jbase + 8 * (i >> 2) + (i & 3);
-        if (j < 0 || j > jmax) s[i] = -INFINITY;
-    }
-}
-
-// One online softmax step over a tile's scores: pr = 2^(s - m), l and O
-// rescaled where m moves.
-template <int D>
-__device__ __forceinline__ void prefill_softmax(const f32x16& s, f32x16 (&o)[D / 32], float& m, float& lsum,
-                                                float (&pr)[16]) {
-    float tmax = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, s[i]);
-    tmax = pair_max(tmax);
-    // Lazy rescale: a column keeps its running max m until a tile's max
-    // exceeds it by more than 8 (log2 units), so P <= 2^8 and O and l are
-    // rescaled only when some column of the wave moves that far (the first
-    // tile with a visible key, then rarely).  The result is the same
-    // softmax: O and l share the scale.
-    if (__any(tmax > m + 8.0f)) {
-        // only the lanes whose max moves rescale (alpha 0 while m = -inf);
-        // the others keep alpha = 1 exactly, also a column with no visible
-        // key yet (m = -inf, where m - m would be NaN)
-        const bool up = tmax > m + 8.0f;
-        const float alpha = up ? __builtin_amdgcn_exp2f(m - tmax) : 1.0f;
-        if (up) m = tmax;
-        lsum *= alpha;
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
-    }
-    const float m_use = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        pr[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
-        lsum += pr[i];
     }
 }
 
@@ -1373,6 +1300,7 @@ static zr_status launch_attn_t(zr_context* ctx, StagedMeta* st, int layer, const
     a.out_f32 = out;
     a.out_bf16 = out_bf16;
     a.out_lo_offset = (ctx->desc.flags & ZR_FLAG_SPLIT_ACTIVATIONS) ? a_plane(st->total_q, ctx->q_cols) : 0;
+    if (zr_status rc = launch_shared_prefix(ctx, st, layer, q)) return rc;
     hipEvent_t ev;
     timing_mark_begin(ctx, kClassAttention, &ev);
     if (st->grid_items > 0) {
@@ -1436,7 +1364,7 @@ static zr_status launch_attn_t(zr_context* ctx, StagedMeta* st, int layer, const
         ZR_LAUNCH_CHECK(ctx);
         timing_mark_end(ctx, kClassOther, ev);
     }
-    return ZR_OK;
+    return launch_shared_merge(ctx, st, out, out_bf16);
 }
 
 // ------------------------------------------------------- any head_dim
@@ -1754,6 +1682,10 @@ zr_status launch_attention_rope(zr_context* ctx, StagedMeta* st, int layer, cons
     if (!st->pure_decode)
         return set_err(ctx, ZR_E_UNSUPPORTED, "RoPE inside attention needs a microbatch of one-row decode sequences");
     if (st->grid_items == 0) return ZR_OK;
+    if (st->n_sunits > 0) {  // shared segments read the rotated q as well: two launches, the same values
+        if (zr_status rc = launch_rope_kv_write(ctx, st, layer, qkv, ctx->q_rope, rope)) return rc;
+        return launch_attention(ctx, st, layer, ctx->q_rope, out, out_bf16);
+    }
     const size_t need = (size_t)st->n_part_items * ctx->local_kv_heads * 16 * (ctx->head_dim + 2);
     if (need > ctx->attn_part_floats)
         return set_err(ctx, ZR_E_OOM, "attention partial workspace too small: need %zu floats, have %zu",

@@ -1,0 +1,84 @@
+// Steps on one tile of scores that the attention kernels over 32-key tiles share
+// (v_mfma_f32_32x32x16_bf16: a lane holds 16 scores of one column, lane l ^ 32
+// the other 16).
+#pragma once
+
+#include "zr_internal.h"
+
+namespace zr {
+
+// x[0..7] as bf16 hi + lo fragments, two values per v_cvt_pk_bf16_f32 (the
+// same bits as split_bf16)
+__device__ inline void split_bf16x8(const float* x, bf16x8& hi, bf16x8& lo) {
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f32x2 v = {x[2 * j], x[2 * j + 1]};
+        const bf16x2 h = __builtin_convertvector(v, bf16x2);
+        const bf16x2 l = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), bf16x2);
+        hi[2 * j] = h[0];
+        hi[2 * j + 1] = h[1];
+        lo[2 * j] = l[0];
+        lo[2 * j + 1] = l[1];
+    }
+}
+
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+
+__device__ inline float pair_max(float x) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ inline float pair_sum(float x) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Scores of keys a column does not see: element i is logical key jbase + 8 (i / 4) + i % 4.
+__device__ __forceinline__ void prefill_mask(f32x16& s, int jbase, int jmax) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int j = jbase + 8 * (i >> 2) + (i & 3);
+        if (j < 0 || j > jmax) s[i] = -INFINITY;
+    }
+}
+
+// One online softmax step over a tile's scores: pr = 2^(s - m), l and O
+// rescaled where m moves.
+template <int D>
+__device__ __forceinline__ void prefill_softmax(const f32x16& s, f32x16 (&o)[D / 32], float& m, float& lsum,
+                                                float (&pr)[16]) {
+    float tmax = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, s[i]);
+    tmax = pair_max(tmax);
+    // Lazy rescale: a column keeps its running max m until a tile's max
+    // exceeds it by more than 8 (log2 units), so P <= 2^8 and O and l are
+    // rescaled only when some column of the wave moves that far (the first
+    // tile with a visible key, then rarely).  The result is the same
+    // softmax: O and l share the scale.
+    if (__any(tmax > m + 8.0f)) {
+        // only the lanes whose max moves rescale (alpha 0 while m = -inf);
+        // the others keep alpha = 1 exactly, also a column with no visible
+        // key yet (m = -inf, where m - m would be NaN)
+        const bool up = tmax > m + 8.0f;
+        const float alpha = up ? __builtin_amdgcn_exp2f(m - tmax) : 1.0f;
+        if (up) m = tmax;
+        lsum *= alpha;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+    }
+    const float m_use = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        pr[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
+        lsum += pr[i];
+    }
+}
+
+}  // namespace zr

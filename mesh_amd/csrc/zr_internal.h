@@ -319,6 +319,11 @@ struct StagedMeta {
                               // inside the decode attention kernel
     bool fuse_rope = false;   // ... and the forward pass has them do so
     bool owns = true;
+    // sequences that share leading pages (attention_shared.hip)
+    int n_segments = 0;       // runs of shared pages
+    int n_sunits = 0;         // work units of the shared-prefix launch (per kv head)
+    int n_smerge = 0;         // query rows whose partials shared_merge_kernel joins
+    int shared_seqs = 0, shared_saved = 0;  // sequences in segments; page reads they save per kv head and launch
     int grid_items = 0;       // decode attention records the launch covers (n_attn_items, or a bucket's
                               // capacity whose records past n_attn_items are empty)
     int grid_merge = 0;       // merge records the launch covers (likewise)
@@ -347,7 +352,14 @@ struct StagedMeta {
     int4* pblocks = nullptr;    // [n_pblocks] {seq, r0, nrows, pages}, most key tiles first (plain layout:
                                 // {seq, first column, columns, pages}, column = row x q heads per kv head + head)
     int4* psplits = nullptr;    // [n_pblocks] {first key tile, end key tile, item, splits}
+    int4* sunits = nullptr;     // [n_sunits][2] {seq, first row in srows, rows | splits << 16, first page},
+                                // {first key tile, end key tile, partial item, end page}
+    int4* smerge = nullptr;     // [n_smerge] {row, first source, sources, 0}
+    int4* ssrc = nullptr;       // partials of a row: {first item, parts, first column of its 16, 0}
+    int* srows = nullptr;       // query rows of the units
     // host copies
+    std::vector<int4> h_sunits, h_smerge, h_ssrc;
+    std::vector<int> h_srows;
     std::vector<int> h_q_len, h_kv_before, h_first_pos, h_first_offset, h_block_tables;
     std::vector<int4> h_items, h_tiles, h_pblocks, h_psplits;
     std::vector<int> h_merge, h_order;
@@ -355,6 +367,16 @@ struct StagedMeta {
     std::vector<uint32_t> h_tokens;
     std::vector<unsigned char> h_blob;
 };
+
+// A run of pages that the block tables of `members` all name at [begin, end).
+struct SharedSegment {
+    int seq, begin, end;      // pages of sequence `seq`'s table
+    std::vector<int> members;
+};
+// The runs of pages that sequences with takes[s] share from the start of their
+// windows, before any new row; cover[s]: the pages of s they hold together.
+void shared_segments(const zr_microbatch* mb, const std::vector<char>& takes, std::vector<SharedSegment>* out,
+                     std::vector<int>* cover);
 
 // A replayed step's bucket: the staged arrays sit at the same offsets of the
 // same device blob every step, sized for the bucket's capacities; records past
@@ -412,6 +434,10 @@ zr_status launch_rope_kv_write(zr_context* ctx, StagedMeta* st, int layer, const
 // out_f32 [T, q_cols] or out_bf16 (A operand of the O projection).
 zr_status launch_attention(zr_context* ctx, StagedMeta* st, int layer, const float* q, float* out_f32,
                            uint16_t* out_bf16);
+// The staged segments' partials, and the join of their rows with the partials of
+// the rows' own pages.
+zr_status launch_shared_prefix(zr_context* ctx, StagedMeta* st, int layer, const float* q);
+zr_status launch_shared_merge(zr_context* ctx, StagedMeta* st, float* out_f32, uint16_t* out_bf16);
 // Plain-layout pools with head_dim a multiple of 4 (tiles staged in pblocks).
 zr_status launch_attention_plain(zr_context* ctx, StagedMeta* st, int layer, const float* q, float* out_f32,
                                  uint16_t* out_bf16);

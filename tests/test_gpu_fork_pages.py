@@ -90,7 +90,7 @@ def decode(backends, tokens):
 
 # every page layout; prompts whose last page is full, has one row, and is the only one
 @pytest.mark.parametrize("kv,heads,kv_heads,d", [("bf16", 4, 2, 64), ("f32", 4, 1, 64), ("bf16", 2, 2, 80)])
-@pytest.mark.parametrize("rows", [5, 32, 33])
+@pytest.mark.parametrize("rows", [5, 32, 33, 100])
 def test_forks_decode_like_sessions_of_their_own(kv, heads, kv_heads, d, rows):
     ctx = model_context(kv, heads, kv_heads, d)
     rng = np.random.default_rng(rows)
