@@ -33,11 +33,9 @@ struct SharedArgs {
 };
 
 // Q^T fragments (B operand) of a column: lane holds Q[col][16 ks + 8 h + j]
-// log2(e) / sqrt(d) as hi + lo (scores come out in log2 units).  hi + lo keeps
-// 16 bits of each value: the rounding of scores of order 1 stays near 2e-6.
+// log2(e) / sqrt(d) in three bf16 parts (scores come out in log2 units).
 template <int D>
-__device__ __forceinline__ void shared_load_q(const float* qp, float scale, bool valid, bf16x8 (&qh)[D / 16],
-                                              bf16x8 (&ql)[D / 16]) {
+__device__ __forceinline__ void shared_load_q(const float* qp, float scale, bool valid, bf16x8 (&q)[D / 16][3]) {
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -49,7 +47,7 @@ __device__ __forceinline__ void shared_load_q(const float* qp, float scale, bool
             x[j] = x0[j] * scale;
             x[4 + j] = x1[j] * scale;
         }
-        split_bf16x8(x, qh[ks], ql[ks]);
+        split3_bf16x8(x, q[ks]);
     }
 }
 
@@ -141,7 +139,9 @@ __device__ __forceinline__ void shared_finish(const SharedArgs& a, f32x16 (&o)[D
 //   S[key][col] = sum_d K[key][d] Q[col][d]; the lane gets key 8 (i / 4) + 4 h + i % 4, i < 16
 //   online softmax per column over the lane's 16 keys and the 16 of lane ^ 32
 //   O[d][col] += sum_key V[key][d] P[key][col]: P's fragment is the lane's own scores
-// Q and P enter as bf16 hi + lo, K and V are exact; sums are f32.
+// Q and P enter in three bf16 parts, which hold all of an f32's 24 bits (two
+// parts, 17 bits, put the result 4e-6 of its norm off: 3.4e-6 from Q, 2.2e-6
+// from P; three leave 1e-7), K and V are exact; sums are f32.
 template <int D, int CW, int KW, int STAGES>
 __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kernel(SharedArgs a,
                                                                               const int* __restrict__ block_tables) {
@@ -217,8 +217,8 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
         }
     tile_pages(kt0 + KW * (STAGES - 1) + slice, npg0, npg1);
     const int grow = a.rows[row0 + (valid ? rloc : 0)];
-    bf16x8 qh[D / 16], ql[D / 16];
-    shared_load_q<D>(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h, a.scale_log2, valid, qh, ql);
+    bf16x8 q[D / 16][3];
+    shared_load_q<D>(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h, a.scale_log2, valid, q);
 
     for (int t = 0; t < nsteps; ++t) {
         ring_wait<VM, STAGES - 2>(min(STAGES - 2, nsteps - 1 - t));
@@ -236,8 +236,9 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
             for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], qh[ks], s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], ql[ks], s, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], q[ks][i], s, 0, 0, 0);
             }
             bf16x8 vf[2][D / 32];
             const bf16x4* sv = (const bf16x4*)st;
@@ -260,13 +261,13 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
             prefill_softmax<D>(s, o, m, lsum, pr);
 #pragma unroll
             for (int ks2 = 0; ks2 < 2; ++ks2) {
-                bf16x8 ph, pl;
-                split_bf16x8(pr + 8 * ks2, ph, pl);
+                bf16x8 p[3];
+                split3_bf16x8(pr + 8 * ks2, p);
 #pragma unroll
-                for (int db = 0; db < D / 32; ++db) {
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], ph, o[db], 0, 0, 0);
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], pl, o[db], 0, 0, 0);
-                }
+                for (int i = 0; i < 3; ++i)
+#pragma unroll
+                    for (int db = 0; db < D / 32; ++db)
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], p[i], o[db], 0, 0, 0);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -275,11 +276,13 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
     shared_finish<D, CW, KW>(a, o, m, lsum, (float*)&lds[0][0][0], slice, wq, lane, kvh, item0, nsplits, valid);
 }
 
-// f32 pools: K, V, Q and P each enter the MFMA as bf16 hi + lo, three products
-// of each pair (the lo x lo one is below 2^-16 of the result).  A tile is split
-// once per workgroup: each wave loads its share of the next tile's f32 runs into
-// registers a step ahead, splits them and stores hi and lo planes in the LDS
-// order of a bf16 tile, two slots deep, one barrier per step.
+// f32 pools: K, V, Q and P each enter the MFMA in three bf16 parts; of the nine
+// products of a pair the six above 2^-24 of the result are formed (two parts and
+// three products are 8e-6 of the result's norm off).  A tile is split once
+// per workgroup: each wave loads its share of the next tile's f32 runs into
+// registers a step ahead, splits them and stores three planes in the LDS order
+// of a bf16 tile, two slots deep, one barrier per step.  At D = 128 the planes
+// and the registers hold one key slice: its waves are alone on their SIMDs.
 template <int D, int CW, int KW>
 __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_kernel(SharedArgs a,
                                                                                   const int* __restrict__ block_tables) {
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
     constexpr int VM = CHUNKS / 64 / CW;  // 512-element runs per wave and tile
     constexpr int RUN = D / 32;
     static_assert(VM * 64 * CW == CHUNKS, "tile copy split");
-    __shared__ bf16x8 lds[2][KW][2][CHUNKS];  // [slot][slice][hi, lo]
+    __shared__ bf16x8 lds[2][KW][3][CHUNKS];  // [slot][slice][part]
     static_assert(shared_combine_bytes(D, CW, KW) <= sizeof(lds), "combine buffer");
 
     const int lane = threadIdx.x & 63;
@@ -336,10 +339,10 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
             const int f = i * CW + wq;
             const float x[8] = {raw[i][0][0], raw[i][0][1], raw[i][0][2], raw[i][0][3],
                                 raw[i][1][0], raw[i][1][1], raw[i][1][2], raw[i][1][3]};
-            bf16x8 hi, lo;
-            split_bf16x8(x, hi, lo);
-            lds[slot][slice][0][f * 64 + lane] = hi;
-            lds[slot][slice][1][f * 64 + lane] = lo;
+            bf16x8 p[3];
+            split3_bf16x8(x, p);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) lds[slot][slice][k][f * 64 + lane] = p[k];
         }
     };
 
@@ -355,8 +358,8 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
     tile_pages(kt0 + KW + slice, npg0, npg1);
     load_raw(pg0, pg1);
     const int grow = a.rows[row0 + (valid ? rloc : 0)];
-    bf16x8 qh[D / 16], ql[D / 16];
-    shared_load_q<D>(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h, a.scale_log2, valid, qh, ql);
+    bf16x8 q[D / 16][3];
+    shared_load_q<D>(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h, a.scale_log2, valid, q);
     store_split(0);
     load_raw(npg0, npg1);
     tile_pages(kt0 + 2 * KW + slice, npg0, npg1);
@@ -376,35 +379,28 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
     };
 
     for (int t = 0; t < nsteps; ++t) {
-        ring_barrier<63>();  // slot t % 2 is written (LDS only: the next tile's loads stay in flight)
+        ring_barrier<63>();  // the slot is written (LDS only: the next tile's loads stay in flight)
         const int kt = kt0 + KW * t + slice;
         if (busy && kt < kt1) {
-            const bf16x8* hi = lds[t & 1][slice][0];
-            const bf16x8* lo = lds[t & 1][slice][1];
+            const bf16x8(&st)[3][CHUNKS] = lds[t & 1][slice];
             const int kbase = ((lane >> 4) & 1) * 2 * (2 * D) + (lane & 15);
             f32x16 s;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {  // K in two batches of dims (registers)
-                bf16x8 kh[D / 32], kl[D / 32];
+            for (int ks = 0; ks < D / 16; ++ks) {
+                bf16x8 k[3];
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const int ks = b * (D / 32) + i;
-                    kh[i] = hi[kbase + (2 * ks + h) * 16];
-                    kl[i] = lo[kbase + (2 * ks + h) * 16];
-                }
+                for (int i = 0; i < 3; ++i) k[i] = st[i][kbase + (2 * ks + h) * 16];
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const int ks = b * (D / 32) + i;
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kh[i], qh[ks], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kh[i], ql[ks], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kl[i], qh[ks], s, 0, 0, 0);
-                }
+                for (int i = 0; i < 3; ++i)
+#pragma unroll
+                    for (int j = 0; j < 3 - i; ++j)
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[j], q[ks][i], s, 0, 0, 0);
             }
             const bool edge = 32 * kt < foff || 32 * kt + 31 > jlast;
             bf16x8 vf[2][D / 32];
-            v_frags(hi, vf);
+            v_frags(st[0], vf);
             __builtin_amdgcn_sched_barrier(0);  // the V reads go out before the softmax
             if (edge) {
                 prefill_mask(s, 32 * kt + 4 * h - foff, jlast - foff);
@@ -412,23 +408,23 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
             }
             float pr[16];
             prefill_softmax<D>(s, o, m, lsum, pr);
-            bf16x8 ph[2], pl[2];
-            split_bf16x8(pr, ph[0], pl[0]);
-            split_bf16x8(pr + 8, ph[1], pl[1]);
+            bf16x8 p[2][3];
+            split3_bf16x8(pr, p[0]);
+            split3_bf16x8(pr + 8, p[1]);
 #pragma unroll
-            for (int ks2 = 0; ks2 < 2; ++ks2)
+            for (int j = 0; j < 3; ++j) {  // part j of V with the parts of P that count
 #pragma unroll
-                for (int db = 0; db < D / 32; ++db) {
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], ph[ks2], o[db], 0, 0, 0);
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], pl[ks2], o[db], 0, 0, 0);
+                for (int ks2 = 0; ks2 < 2; ++ks2)
+#pragma unroll
+                    for (int i = 0; i < 3 - j; ++i)
+#pragma unroll
+                        for (int db = 0; db < D / 32; ++db)
+                            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], p[ks2][i], o[db], 0, 0, 0);
+                if (j < 2) {
+                    v_frags(st[j + 1], vf);
+                    if (edge) shared_mask_v<D>(vf, 32 * kt - foff, h, jlast - foff);
                 }
-            v_frags(lo, vf);
-            if (edge) shared_mask_v<D>(vf, 32 * kt - foff, h, jlast - foff);
-#pragma unroll
-            for (int ks2 = 0; ks2 < 2; ++ks2)
-#pragma unroll
-                for (int db = 0; db < D / 32; ++db)
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], ph[ks2], o[db], 0, 0, 0);
+            }
         }
         if (t + 1 < nsteps) {
             store_split((t + 1) & 1);  // last read in step t - 1, a barrier ago
@@ -516,11 +512,13 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const float* __restri
 
 template <int D>
 static void launch_units(zr_context* ctx, StagedMeta* st, const SharedArgs& a) {
-    const dim3 grid(st->n_sunits * ctx->local_kv_heads), block(512);
+    const dim3 grid(st->n_sunits * ctx->local_kv_heads);
+    constexpr int KW = D == 64 ? 2 : 1;
     if (ctx->desc.kv_dtype == ZR_DTYPE_BF16)
-        hipLaunchKernelGGL((shared_prefix_kernel<D, 4, 2, 3>), grid, block, 0, ctx->stream, a, st->block_tables);
+        hipLaunchKernelGGL((shared_prefix_kernel<D, 4, 2, 3>), grid, dim3(512), 0, ctx->stream, a, st->block_tables);
     else
-        hipLaunchKernelGGL((shared_prefix_f32_kernel<D, 4, 2>), grid, block, 0, ctx->stream, a, st->block_tables);
+        hipLaunchKernelGGL((shared_prefix_f32_kernel<D, 4, KW>), grid, dim3(256 * KW), 0, ctx->stream, a,
+                           st->block_tables);
 }
 
 zr_status launch_shared_prefix(zr_context* ctx, StagedMeta* st, int layer, const float* q) {

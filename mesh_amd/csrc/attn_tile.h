@@ -24,6 +24,25 @@ __device__ inline void split_bf16x8(const float* x, bf16x8& hi, bf16x8& lo) {
     }
 }
 
+// x[0..7] as three bf16 fragments whose sum is x to its last f32 bit (8 bits
+// each; a remainder is exact in f32, so only the third part is rounded away
+// from x, below 2^-25 of it)
+__device__ inline void split3_bf16x8(const float* x, bf16x8 (&p)[3]) {
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f32x2 v = {x[2 * j], x[2 * j + 1]};
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const bf16x2 h = __builtin_convertvector(v, bf16x2);
+            if (k < 2) v -= __builtin_convertvector(h, f32x2);
+            p[k][2 * j] = h[0];
+            p[k][2 * j + 1] = h[1];
+        }
+    }
+}
+
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 
 __device__ inline float pair_max(float x) {
