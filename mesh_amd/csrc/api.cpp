@@ -475,20 +475,27 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     st->h_ssrc.clear();
     st->h_srows.clear();
     st->n_segments = (int)segments.size();
-    st->shared_seqs = st->shared_saved = 0;
+    st->shared_seqs = st->shared_rows = st->shared_saved = 0;
     std::vector<std::vector<int4>> row_src;  // by query row: partials {first item, parts, first column of its 16}
     std::vector<int> cu_rows(S + 1, 0);
     for (int s = 0; s < S; ++s) cu_rows[s + 1] = cu_rows[s] + mb->q_len[s];
     if (!segments.empty()) {
         row_src.resize(total_q);
-        const int upr = 128 / G, gpr = 16 / G;  // rows per unit and per 16-column group
-        long unit_tiles = 0;
-        for (const SharedSegment& g : segments) {
+        auto rows_of = [&](const SharedSegment& g) {
             int rows = 0;
             for (int s : g.members) rows += mb->q_len[s];
-            unit_tiles += (long)((rows + upr - 1) / upr) * ((g.end - g.begin + 1) / 2);
-        }
-        const int unit_tps = (int)std::max<long>(4, (unit_tiles * ctx->local_kv_heads + slots - 1) / slots);
+            return rows;
+        };
+        int most = 0;
+        for (const SharedSegment& g : segments) most = std::max(most, rows_of(g));
+        st->unit_cols = f32_kv || most * G > 64 ? 128 : most * G > 32 ? 64 : 32;
+        const int upr = st->unit_cols / G, gpr = 16 / G;  // rows per unit and per 16-column group
+        const int slices = 128 / st->unit_cols;           // tiles a unit takes at once
+        long unit_steps = 0;
+        for (const SharedSegment& g : segments)
+            unit_steps += (long)((rows_of(g) + upr - 1) / upr) * (((g.end - g.begin + 1) / 2 + slices - 1) / slices);
+        const int unit_tps =
+            slices * (int)std::max<long>(2, (unit_steps * ctx->local_kv_heads + 511) / 512);
         for (const SharedSegment& g : segments) {
             const int row0 = (int)st->h_srows.size();
             for (int s : g.members)
@@ -499,7 +506,8 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
             for (int sp = 0; sp < ns; ++sp)  // the units of a run of tiles side by side: they read the same pages
                 for (int r = 0; r < rows; r += upr) {
                     const int n = std::min(upr, rows - r);
-                    st->h_sunits.push_back(make_int4(g.seq, row0 + r, n | ns << 16, g.begin));
+                    const unsigned foff = g.begin == 0 ? mb->first_offset[g.seq] : 0;
+                    st->h_sunits.push_back(make_int4((int)(g.seq | foff << 27), row0 + r, n | ns << 16, g.begin));
                     st->h_sunits.push_back(make_int4((int)((long)sp * nt / ns), (int)((long)(sp + 1) * nt / ns),
                                                      next_item + (r / gpr) * ns + sp, g.end));
                 }
@@ -511,15 +519,17 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
         // ... and the partials of the rows' own pages
         for (int t = 0; t < n_decode_tiles; ++t) {
             const int4 tl = st->h_tiles[t];
-            if (!cover[tl.x]) continue;
             for (int i = 0; i < tl.z; ++i)
                 row_src[cu_rows[tl.x] + tl.y + i].push_back(make_int4(tl.w, st->h_tiles[t + 1].w - tl.w, i * G, 0));
         }
         for (int s = 0; s < S; ++s) {
-            if (!cover[s]) continue;
-            ++st->shared_seqs;
+            st->shared_seqs += cover[s] > 0;
+            st->shared_rows += cover[s] > 0 ? mb->q_len[s] : 0;
+            if (as_prefill(s)) continue;
             for (int r = cu_rows[s]; r < cu_rows[s + 1]; ++r) {
-                st->h_smerge.push_back(make_int4(r, (int)st->h_ssrc.size(), (int)row_src[r].size(), 0));
+                int parts = 0;
+                for (const int4& x : row_src[r]) parts += x.y;
+                st->h_smerge.push_back(make_int4(r, (int)st->h_ssrc.size(), (int)row_src[r].size(), parts));
                 st->h_ssrc.insert(st->h_ssrc.end(), row_src[r].begin(), row_src[r].end());
             }
         }
@@ -536,7 +546,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     // tiles whose splits need the merge kernel (every prefill group tile has several)
     st->h_merge.clear();
     for (int t = 0; t < st->n_tiles; ++t)
-        if (t >= n_decode_tiles || (st->h_tiles[t + 1].w - st->h_tiles[t].w > 1 && !cover[st->h_tiles[t].x]))
+        if (t >= n_decode_tiles || (st->h_tiles[t + 1].w - st->h_tiles[t].w > 1 && segments.empty()))
             st->h_merge.push_back(t);
     st->n_merge = (int)st->h_merge.size();
     // Per-launch records in the order the kernels read them, so that a
@@ -554,7 +564,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
             const int first = tl.w, end = st->h_tiles[it.x + 1].w;
             const int seq = tl.x;
             unsigned meta = (unsigned)item;
-            if (end - first == 1 && !cover[seq]) meta |= kAttnSingle;
+            if (end - first == 1 && segments.empty()) meta |= kAttnSingle;
             if (item == end - 1) meta |= kAttnLast;
             const int* bt = mb->block_tables + (size_t)seq * stride;
             auto pid = [&](int k) { return it.y + k < it.z ? bt[it.y + k] : 0; };
@@ -1131,7 +1141,7 @@ zr_status zr_staged_prefix_info(const zr_staged* s, zr_prefix_info* out) {
     if (!st || !out) return set_global_err(ZR_E_INVALID, "null argument");
     out->segments = st->n_segments;
     out->sequences = st->shared_seqs;
-    out->rows = st->n_smerge;
+    out->rows = st->shared_rows;
     out->units = st->n_sunits;
     out->pages_saved = st->shared_saved;
     return ZR_OK;

@@ -36,51 +36,6 @@ namespace zr {
 
 __device__ inline float shfl_xor(float v, int mask) { return __shfl_xor(v, mask, 64); }
 
-// Every page of the pool is read once per launch (one workgroup per kv head
-// and page run), so the loads carry the nontemporal hint: the lines are
-// streamed through L2 with low retention instead of displacing what the other
-// waves on the XCD still read (256-session Llama-3-8B step: attention 9.55-9.78
-// -> 8.81-8.99 ms per step; 32-session TinyLlama step unchanged).
-template <typename KV, int D> struct PageRegs;
-
-// bf16 pool: K fragment per 32 dims = 8 bf16 (16 B); V per 32 dims = 8 bf16
-// (16 B): tokens 4 q4 .. 4 q4 + 3 of dims 32 vb + c, then of 32 vb + 16 + c.
-// Both are one 1 KiB contiguous wave load.
-template <int D> struct PageRegs<uint16_t, D> {
-    bf16x8 k[D / 32];
-    bf16x8 v[D / 32];
-    __device__ inline void load(const uint16_t* kp, const uint16_t* vp, int lane) {
-#pragma unroll
-        for (int kb = 0; kb < D / 32; ++kb)
-            k[kb] = __builtin_nontemporal_load((const bf16x8*)(kp + ((size_t)kb * kWave + lane) * 8));
-#pragma unroll
-        for (int vb = 0; vb < D / 32; ++vb)
-            v[vb] = __builtin_nontemporal_load((const bf16x8*)(vp + ((size_t)vb * kWave + lane) * 8));
-    }
-};
-
-// f32 pool (page_order): the same 8 values per lane and 32 dims, as two
-// 16 B halves that each come from one contiguous 1 KiB wave run (K: dims
-// 8 g + [0, 4) then + [4, 8); V: dim d then d + 16, 4 tokens each).
-template <int D> struct PageRegs<float, D> {
-    f32x4 k[D / 32][2];
-    f32x4 v[D / 32][2];
-    __device__ inline void load(const float* kp, const float* vp, int lane) {
-#pragma unroll
-        for (int kb = 0; kb < D / 32; ++kb) {
-            const f32x4* src = (const f32x4*)(kp + (size_t)kb * kWave * 8) + lane;
-            k[kb][0] = __builtin_nontemporal_load(src);
-            k[kb][1] = __builtin_nontemporal_load(src + kWave);
-        }
-#pragma unroll
-        for (int vb = 0; vb < D / 32; ++vb) {
-            const f32x4* src = (const f32x4*)(vp + (size_t)vb * kWave * 8) + lane;
-            v[vb][0] = __builtin_nontemporal_load(src);
-            v[vb][1] = __builtin_nontemporal_load(src + kWave);
-        }
-    }
-};
-
 __device__ inline bf16x4 to_bf16x4(const float* x, bool lo_part) {
     bf16x4 r;
 #pragma unroll
@@ -156,83 +111,6 @@ __device__ inline void pv_mfma2(const PageRegs<float, D>& pa, const PageRegs<flo
     }
 }
 
-// The same products at f32's own precision, for rows whose other pages run in
-// shared_prefix_kernel (attention_shared.hip): Q and P in three bf16 parts, and
-// f32 pools' K and V too, where of the nine products the six above 2^-24 of the
-// result are formed.  The launch is bound by its pages; the MFMAs hide.
-template <int D>
-__device__ inline f32x4 qk3_mfma(const PageRegs<uint16_t, D>& pg, const bf16x8 (*q)[D / 32][64], int lane) {
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int kb = 0; kb < D / 32; ++kb)
-#pragma unroll
-        for (int i = 0; i < 3; ++i) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pg.k[kb], q[i][kb][lane], s, 0, 0, 0);
-    return s;
-}
-
-template <int D>
-__device__ inline f32x4 qk3_mfma(const PageRegs<float, D>& pg, const bf16x8 (*q)[D / 32][64], int lane) {
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int kb = 0; kb < D / 32; ++kb) {
-        float kf[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            kf[j] = pg.k[kb][0][j];
-            kf[4 + j] = pg.k[kb][1][j];
-        }
-        bf16x8 k[3];
-        split3_bf16x8(kf, k);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const bf16x8 qi = q[i][kb][lane];
-#pragma unroll
-            for (int j = 0; j < 3 - i; ++j) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j], qi, s, 0, 0, 0);
-        }
-    }
-    return s;
-}
-
-template <int D>
-__device__ inline void pv3_mfma2(const PageRegs<uint16_t, D>& pa, const PageRegs<uint16_t, D>& pb, const bf16x8 (&p)[3],
-                                 f32x4* o) {
-#pragma unroll
-    for (int vb = 0; vb < D / 32; ++vb) {
-        const bf16x8 v0 = __builtin_shufflevector(pa.v[vb], pb.v[vb], 0, 1, 2, 3, 8, 9, 10, 11);
-        const bf16x8 v1 = __builtin_shufflevector(pa.v[vb], pb.v[vb], 4, 5, 6, 7, 12, 13, 14, 15);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            o[2 * vb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, p[i], o[2 * vb], 0, 0, 0);
-            o[2 * vb + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, p[i], o[2 * vb + 1], 0, 0, 0);
-        }
-    }
-}
-
-template <int D>
-__device__ inline void pv3_mfma2(const PageRegs<float, D>& pa, const PageRegs<float, D>& pb, const bf16x8 (&p)[3],
-                                 f32x4* o) {
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db) {
-        const f32x4 va = pa.v[db >> 1][db & 1], vbv = pb.v[db >> 1][db & 1];
-        const float vf[8] = {va[0], va[1], va[2], va[3], vbv[0], vbv[1], vbv[2], vbv[3]};
-        bf16x8 v[3];
-        split3_bf16x8(vf, v);
-#pragma unroll
-        for (int i = 0; i < 3; ++i)
-#pragma unroll
-            for (int j = 0; j < 3 - i; ++j) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[j], p[i], o[db], 0, 0, 0);
-    }
-}
-
-// max over the lanes {l, l^16, l^32, l^48} (the four quads holding one column),
-// with gfx950's VALU lane swaps.
-__device__ inline float quad_max(float x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 struct AttnArgs {
     const float* q;          // [T, q_cols]
     int q_cols;
@@ -263,7 +141,7 @@ struct AttnArgs {
     const float2* rope_cs;   // [T][D / 2] (cos, sin), or null: no rotation
 };
 
-template <typename KV, int D, int RING, bool FUSE, int PARTS = 2>
+template <typename KV, int D, int RING, bool FUSE>
 __global__ __launch_bounds__(64) void paged_attention_kernel(AttnArgs a) {
     const int lane = threadIdx.x;
     // Workgroups go to the 8 XCDs round-robin (XCD = blockIdx % 8).  Block
@@ -288,9 +166,8 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(AttnArgs a) {
     const int jmax = r1.y + (col_valid ? qi : 0);
 
     // Q^T as the MFMA B operand (lane holds Q[c][32*kb + 8*q4 + j]) as bf16
-    // hi + lo fragments (PARTS = 3: three), parked in LDS to keep registers for the
-    // page ring.
-    __shared__ bf16x8 qs[PARTS][D / 32][64];
+    // hi + lo fragments, parked in LDS to keep registers for the page ring.
+    __shared__ bf16x8 qs[2][D / 32][64];
     const bf16x8* qhi = qs[0][0];
     const bf16x8* qlo = qs[1][0];
 
@@ -307,14 +184,8 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(AttnArgs a) {
     // a page pair (p, p + 1): S^T = K Q^T for both, one online-softmax step
     // over 32 tokens, O^T += V^T P^T.  has_b == false masks page B (odd tail).
     auto process2 = [&](const PageRegs<KV, D>& pa, const PageRegs<KV, D>& pb, int p, bool has_b) {
-        f32x4 sa, sb;
-        if constexpr (PARTS == 3) {
-            sa = qk3_mfma<D>(pa, qs, lane);
-            sb = qk3_mfma<D>(pb, qs, lane);
-        } else {
-            sa = qk_mfma<D>(pa, qhi, qlo, lane);
-            sb = qk_mfma<D>(pb, qhi, qlo, lane);
-        }
+        const f32x4 sa = qk_mfma<D>(pa, qhi, qlo, lane);
+        const f32x4 sb = qk_mfma<D>(pb, qhi, qlo, lane);
         float sc[8];
         float pmax = -INFINITY;
         const int jbase = p * kPageRows + q4 * 4 - foff;
@@ -343,13 +214,7 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(AttnArgs a) {
         for (int db = 0; db < D / 16; ++db)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[db][i] *= alpha;
-        if constexpr (PARTS == 3) {
-            bf16x8 p3[3];
-            split3_bf16x8(pr, p3);
-            pv3_mfma2<D>(pa, pb, p3, o);
-        } else {
-            pv_mfma2<D>(pa, pb, to_bf16x8(pr, false), to_bf16x8(pr, true), o);
-        }
+        pv_mfma2<D>(pa, pb, to_bf16x8(pr, false), to_bf16x8(pr, true), o);
     };
 
     // Register ring of RING page sets, consumed in pairs: RING - 2 pages are
@@ -551,15 +416,8 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(AttnArgs a) {
     for (int kb = 0; kb < D / 32; ++kb) {
         const float x[8] = {qx[kb][0][0], qx[kb][0][1], qx[kb][0][2], qx[kb][0][3],
                             qx[kb][1][0], qx[kb][1][1], qx[kb][1][2], qx[kb][1][3]};
-        if constexpr (PARTS == 3) {
-            bf16x8 q3[3];
-            split3_bf16x8(x, q3);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) qs[i][kb][lane] = q3[i];
-        } else {
-            qs[0][kb][lane] = to_bf16x8(x, false);
-            qs[1][kb][lane] = to_bf16x8(x, true);
-        }
+        qs[0][kb][lane] = to_bf16x8(x, false);
+        qs[1][kb][lane] = to_bf16x8(x, true);
     }
     for (int p = page_b; p < pend; p += RING) {
 #pragma unroll
@@ -1388,18 +1246,17 @@ static zr_status launch_attn_t(zr_context* ctx, StagedMeta* st, int layer, const
     a.out_f32 = out;
     a.out_bf16 = out_bf16;
     a.out_lo_offset = (ctx->desc.flags & ZR_FLAG_SPLIT_ACTIVATIONS) ? a_plane(st->total_q, ctx->q_cols) : 0;
-    if (zr_status rc = launch_shared_prefix(ctx, st, layer, q)) return rc;
+    // with shared segments one launch takes them and every decode tile
+    if (st->n_sunits > 0)
+        if (zr_status rc = launch_shared_attention(ctx, st, layer, q)) return rc;
     hipEvent_t ev;
     timing_mark_begin(ctx, kClassAttention, &ev);
-    if (st->grid_items > 0) {
+    if (st->grid_items > 0 && st->n_sunits == 0) {
         // bf16 pages: a 6-page ring, one wave per SIMD (measured: a 4-page ring
         // at two waves per SIMD spills and loses ~20%); f32 pages: 4 pages
         const dim3 grid(((st->grid_items + 7) / 8) * 8 * ctx->local_kv_heads);
         if (qkv)
             hipLaunchKernelGGL((paged_attention_kernel<KV, D, sizeof(KV) == 4 ? 4 : 6, true>), grid, dim3(64), 0,
-                               ctx->stream, a);
-        else if (st->n_sunits > 0)
-            hipLaunchKernelGGL((paged_attention_kernel<KV, D, sizeof(KV) == 4 ? 4 : 6, false, 3>), grid, dim3(64), 0,
                                ctx->stream, a);
         else
             hipLaunchKernelGGL((paged_attention_kernel<KV, D, sizeof(KV) == 4 ? 4 : 6, false>), grid, dim3(64), 0,

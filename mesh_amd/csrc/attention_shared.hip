@@ -9,8 +9,12 @@
 // all of their rows see all of them.  Over disjoint key sets i the softmax
 // splits into (m_i, l_i, o_i) = (max s, sum 2^(s - m_i), sum 2^(s - m_i) v):
 //   M = max m_i,  o = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
-// Segments run here, the pages after them in paged_attention_kernel's tiles,
-// and shared_merge_kernel joins the partials of a row.
+// One launch takes the segments (units) and every decode tile's own pages
+// (tails) and leaves partials; shared_merge_kernel joins those of a row.
+//
+// A unit is bound by the MFMAs (each page serves up to 128 columns), a tail by
+// its pages, so the two kinds of workgroup alternate in dispatch order and run
+// side by side on a CU: two of 4 waves each.
 #include "attn_tile.h"
 #include "zr_internal.h"
 
@@ -21,12 +25,14 @@ struct SharedArgs {
     int q_cols;
     const void* pool;     // layer base of the pool
     size_t page_elems;
-    int stride;           // block table row stride
-    const int* first_offset;
-    const int4* units;    // two records per work unit: {seq, first of its rows in `rows`, rows | splits << 16, first page},
-                          // {first key tile, end key tile, partial item, end page}
+    int stride;           // block table row stride (the table is a kernel argument)
+    const int4* units;    // two records per work unit: {seq | first row of its first page << 27, first of its rows in
+                          // `rows`, rows | splits << 16, first page}, {first key tile, end key tile, partial item,
+                          // end page}
     const int* rows;      // query rows of the microbatch
-    int n_units;
+    const int4* rec;      // three records per tail, longest first (AttnArgs::rec)
+    int n_units, n_tails;
+    int unit_groups, groups;  // of 8 workgroups: those of units, all
     int G, kv_heads;
     float scale_log2;     // log2(e) / sqrt(d)
     float* part;          // [items][kv_heads][16][D + 2]
@@ -34,22 +40,43 @@ struct SharedArgs {
 
 // Q^T fragments (B operand) of a column: lane holds Q[col][16 ks + 8 h + j]
 // log2(e) / sqrt(d) in three bf16 parts (scores come out in log2 units).
-template <int D>
-__device__ __forceinline__ void shared_load_q(const float* qp, float scale, bool valid, bf16x8 (&q)[D / 16][3]) {
+template <int D> struct SharedQ {
+    f32x4 x[D / 16][2];
+    __device__ __forceinline__ void load(const float* qp) {
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        const f32x4 x0 = valid ? *(const f32x4*)(qp + 16 * ks) : zero;
-        const f32x4 x1 = valid ? *(const f32x4*)(qp + 16 * ks + 4) : zero;
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[j] = x0[j] * scale;
-            x[4 + j] = x1[j] * scale;
+        for (int ks = 0; ks < D / 16; ++ks) {
+            x[ks][0] = *(const f32x4*)(qp + 16 * ks);
+            x[ks][1] = *(const f32x4*)(qp + 16 * ks + 4);
         }
-        split3_bf16x8(x, q[ks]);
     }
-}
+    __device__ __forceinline__ void split(float scale, bf16x8 (&q)[D / 16][3]) const {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = x[ks][j >> 2][j & 3] * scale;
+            split3_bf16x8(y, q[ks]);
+        }
+    }
+};
+
+// A unit's page ids, 64 at a time, one per lane: a tile's two come by lane reads,
+// so that no table load stands before its copies.  Tiles are asked for in order;
+// one past the segment's end repeats its last page.
+struct SharedPages {
+    const int* bt;   // the sequence's table from the unit's first page on
+    int last;        // last page of the segment, counted from there
+    int base, ids;
+    __device__ __forceinline__ void fetch(int lane) { ids = bt[min(base + lane, last)]; }
+    __device__ __forceinline__ void tile(int rel, int lane, int& pg0, int& pg1) {
+        if (2 * rel >= base + 64) {
+            base = (2 * rel) & ~63;
+            fetch(lane);
+        }
+        pg0 = __builtin_amdgcn_readlane(ids, 2 * rel - base);
+        pg1 = __builtin_amdgcn_readlane(ids, 2 * rel - base + 1);
+    }
+};
 
 // V rows of keys outside [0, last] enter the product as 0: their weights are 0,
 // but 0 x inf is NaN, and rows before a trimmed window hold whatever they held.
@@ -142,23 +169,25 @@ __device__ __forceinline__ void shared_finish(const SharedArgs& a, f32x16 (&o)[D
 // Q and P enter in three bf16 parts, which hold all of an f32's 24 bits (two
 // parts, 17 bits, put the result 4e-6 of its norm off: 3.4e-6 from Q, 2.2e-6
 // from P; three leave 1e-7), K and V are exact; sums are f32.
+constexpr size_t unit_lds(int D, int KW, int stages) { return (size_t)stages * KW * 8 * D * 16; }
+
 template <int D, int CW, int KW, int STAGES>
-__global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kernel(SharedArgs a,
-                                                                              const int* __restrict__ block_tables) {
+__device__ __forceinline__ void shared_unit(const SharedArgs& a, const int* __restrict__ block_tables, int wg, bf16x8* buf) {
     constexpr int CHUNKS = 8 * D;        // 16 B chunks per tile: 2 pages x (K, V) x 16 rows x D bf16
     constexpr int VM = CHUNKS / 64 / CW; // copies (1 KiB each) per wave and tile
     constexpr int RUN = D / 32;          // 1 KiB runs of one head's K (or V) page
     static_assert(VM * 64 * CW == CHUNKS, "tile copy split");
-    __shared__ bf16x8 lds[STAGES][KW][CHUNKS];
-    static_assert(shared_combine_bytes(D, CW, KW) <= sizeof(lds), "combine buffer");
+    static_assert(shared_combine_bytes(D, CW, KW) <= unit_lds(D, KW, STAGES), "combine buffer");
+    auto lds = [&](int slot, int slice) { return buf + (size_t)(slot * KW + slice) * CHUNKS; };
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slice = wave / CW, wq = wave - slice * CW;
-    const int rank = __builtin_amdgcn_readfirstlane(blockIdx.x / a.kv_heads);
-    const int kvh = blockIdx.x - rank * a.kv_heads;
+    const int rank = __builtin_amdgcn_readfirstlane(wg / a.kv_heads);
+    const int kvh = wg - rank * a.kv_heads;
+    if (rank >= a.n_units) return;
     const int4 u0 = a.units[2 * rank], u1 = a.units[2 * rank + 1];
-    const int seq = __builtin_amdgcn_readfirstlane(u0.x), row0 = __builtin_amdgcn_readfirstlane(u0.y);
+    const int seq = __builtin_amdgcn_readfirstlane(u0.x) & 0x7ffffff, row0 = __builtin_amdgcn_readfirstlane(u0.y);
     const int nrows = __builtin_amdgcn_readfirstlane(u0.z & 0xffff), nsplits = __builtin_amdgcn_readfirstlane(u0.z >> 16);
     const int pb = __builtin_amdgcn_readfirstlane(u0.w), pe = __builtin_amdgcn_readfirstlane(u1.w);
     const int kt0 = __builtin_amdgcn_readfirstlane(u1.x), kt1 = __builtin_amdgcn_readfirstlane(u1.y);
@@ -170,18 +199,16 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
     const bool valid = rloc < nrows;
     const bool busy = wq * 32 < nrows * a.G;  // the wave has a column
     // keys of the segment's first page before the window, and of its last tile past its end
-    const int foff = pb == 0 ? __builtin_amdgcn_readfirstlane(a.first_offset[seq]) : 0;
+    const int foff = __builtin_amdgcn_readfirstlane((unsigned)u0.x >> 27);
     const int jlast = (pe - pb) * kPageRows - 1;
 
     const uint16_t* pool = (const uint16_t*)a.pool;
-    const int* bt = block_tables + (size_t)seq * a.stride;
+    const int p0 = pb + 2 * kt0;  // the unit's first page
+    SharedPages pages{block_tables + (size_t)seq * a.stride + p0, pe - 1 - p0, 0, 0};
+    pages.fetch(lane);
+    const int grow = a.rows[row0 + (valid ? rloc : 0)];  // (columns past the unit's rows compute its first row, unused)
     const size_t kv_tile = (size_t)kPageRows * D;
     const size_t v_block = (size_t)a.kv_heads * kv_tile;
-    // pool pages of tile kt (a tile past the segment's end repeats its last page)
-    auto tile_pages = [&](int kt, int& pg0, int& pg1) {
-        pg0 = __builtin_amdgcn_readfirstlane(bt[min(pb + 2 * kt, pe - 1)]);
-        pg1 = __builtin_amdgcn_readfirstlane(bt[min(pb + 2 * kt + 1, pe - 1)]);
-    };
     const uint32_t page_bytes = (uint32_t)(a.page_elems * 2);
     const int voff = lane * 16;
     auto issue = [&](int slot, int pg0, int pg1) {
@@ -194,7 +221,7 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
             const int f = i * CW + wq;  // (page, K or V, 1 KiB run)
             const int pp = f / (2 * RUN), kv = (f / RUN) & 1, run = f % RUN;
             const int soff = (int)(((kv ? v_block : 0) + (size_t)kvh * kv_tile) * 2) + run * 1024;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(pp ? r1 : r0, (lds_void*)&lds[slot][slice][f * 64], 16, voff, soff,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(pp ? r1 : r0, (lds_void*)(lds(slot, slice) + f * 64), 16, voff, soff,
                                                      0, 0);
         }
     };
@@ -206,26 +233,31 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
         for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
     float m = -INFINITY, lsum = 0.0f;
 
-    // step p holds tile kt0 + KW p + slice
+    // step p holds tile kt0 + KW p + slice; the rows' Q goes out behind the first
+    // step's copies
     const int nsteps = (kt1 - kt0 + KW - 1) / KW;
-    int npg0 = 0, npg1 = 0;
+    SharedQ<D> qx;
+    int pg0, pg1;
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s)
+    for (int s = 0; s < STAGES - 1; ++s) {
         if (s < nsteps) {
-            tile_pages(kt0 + KW * s + slice, npg0, npg1);
-            issue(s, npg0, npg1);
+            pages.tile(KW * s + slice, lane, pg0, pg1);
+            issue(s, pg0, pg1);
         }
-    tile_pages(kt0 + KW * (STAGES - 1) + slice, npg0, npg1);
-    const int grow = a.rows[row0 + (valid ? rloc : 0)];
+        if (s == 0) qx.load(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h);
+    }
     bf16x8 q[D / 16][3];
-    shared_load_q<D>(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h, a.scale_log2, valid, q);
+    qx.split(a.scale_log2, q);
 
     for (int t = 0; t < nsteps; ++t) {
         ring_wait<VM, STAGES - 2>(min(STAGES - 2, nsteps - 1 - t));
-        if (t + STAGES - 1 < nsteps) issue((t + STAGES - 1) % STAGES, npg0, npg1);
+        if (t + STAGES - 1 < nsteps) {
+            pages.tile(KW * (t + STAGES - 1) + slice, lane, pg0, pg1);
+            issue((t + STAGES - 1) % STAGES, pg0, pg1);
+        }
         const int kt = kt0 + KW * t + slice;
         if (busy && kt < kt1) {
-            const bf16x8* st = lds[t % STAGES][slice];
+            const bf16x8* st = lds(t % STAGES, slice);
             const int kbase = ((lane >> 4) & 1) * 2 * (2 * D) + (lane & 15);  // page (l % 32) / 16, row l % 16
             bf16x8 kf[D / 16];
 #pragma unroll
@@ -270,10 +302,8 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
                         o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], p[i], o[db], 0, 0, 0);
             }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (t + STAGES - 1 < nsteps) tile_pages(kt0 + KW * (t + STAGES) + slice, npg0, npg1);
     }
-    shared_finish<D, CW, KW>(a, o, m, lsum, (float*)&lds[0][0][0], slice, wq, lane, kvh, item0, nsplits, valid);
+    shared_finish<D, CW, KW>(a, o, m, lsum, (float*)buf, slice, wq, lane, kvh, item0, nsplits, valid);
 }
 
 // f32 pools: K, V, Q and P each enter the MFMA in three bf16 parts; of the nine
@@ -281,25 +311,27 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_kerne
 // three products are 8e-6 of the result's norm off).  A tile is split once
 // per workgroup: each wave loads its share of the next tile's f32 runs into
 // registers a step ahead, splits them and stores three planes in the LDS order
-// of a bf16 tile, two slots deep, one barrier per step.  At D = 128 the planes
-// and the registers hold one key slice: its waves are alone on their SIMDs.
-template <int D, int CW, int KW>
-__global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_kernel(SharedArgs a,
-                                                                                  const int* __restrict__ block_tables) {
+// of a bf16 tile, two slots deep, one barrier per step.
+constexpr size_t unit_f32_lds(int D) { return (size_t)2 * 3 * 8 * D * 16; }
+
+template <int D>
+__device__ __forceinline__ void shared_unit_f32(const SharedArgs& a, const int* __restrict__ block_tables, int wg,
+                                                bf16x8* buf) {
+    constexpr int CW = 4, KW = 1;
     constexpr int CHUNKS = 8 * D;         // 16 B chunks per plane of a tile
     constexpr int VM = CHUNKS / 64 / CW;  // 512-element runs per wave and tile
     constexpr int RUN = D / 32;
     static_assert(VM * 64 * CW == CHUNKS, "tile copy split");
-    __shared__ bf16x8 lds[2][KW][3][CHUNKS];  // [slot][slice][part]
-    static_assert(shared_combine_bytes(D, CW, KW) <= sizeof(lds), "combine buffer");
+    auto lds = [&](int slot, int part) { return buf + (size_t)(slot * 3 + part) * CHUNKS; };
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slice = wave / CW, wq = wave - slice * CW;
-    const int rank = __builtin_amdgcn_readfirstlane(blockIdx.x / a.kv_heads);
-    const int kvh = blockIdx.x - rank * a.kv_heads;
+    const int rank = __builtin_amdgcn_readfirstlane(wg / a.kv_heads);
+    const int kvh = wg - rank * a.kv_heads;
+    if (rank >= a.n_units) return;
     const int4 u0 = a.units[2 * rank], u1 = a.units[2 * rank + 1];
-    const int seq = __builtin_amdgcn_readfirstlane(u0.x), row0 = __builtin_amdgcn_readfirstlane(u0.y);
+    const int seq = __builtin_amdgcn_readfirstlane(u0.x) & 0x7ffffff, row0 = __builtin_amdgcn_readfirstlane(u0.y);
     const int nrows = __builtin_amdgcn_readfirstlane(u0.z & 0xffff), nsplits = __builtin_amdgcn_readfirstlane(u0.z >> 16);
     const int pb = __builtin_amdgcn_readfirstlane(u0.w), pe = __builtin_amdgcn_readfirstlane(u1.w);
     const int kt0 = __builtin_amdgcn_readfirstlane(u1.x), kt1 = __builtin_amdgcn_readfirstlane(u1.y);
@@ -310,17 +342,16 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
     const int rloc = c / a.G, g = c - rloc * a.G;
     const bool valid = rloc < nrows;
     const bool busy = wq * 32 < nrows * a.G;
-    const int foff = pb == 0 ? __builtin_amdgcn_readfirstlane(a.first_offset[seq]) : 0;
+    const int foff = __builtin_amdgcn_readfirstlane((unsigned)u0.x >> 27);
     const int jlast = (pe - pb) * kPageRows - 1;
 
-    const int* bt = block_tables + (size_t)seq * a.stride;
+    const int p0 = pb + 2 * kt0;
+    SharedPages pages{block_tables + (size_t)seq * a.stride + p0, pe - 1 - p0, 0, 0};
+    pages.fetch(lane);
+    const int grow = a.rows[row0 + (valid ? rloc : 0)];
     const size_t kv_tile = (size_t)kPageRows * D;
     const size_t v_block = (size_t)a.kv_heads * kv_tile;
     const float* pool = (const float*)a.pool + (size_t)kvh * kv_tile + 4 * lane;
-    auto tile_pages = [&](int kt, int& pg0, int& pg1) {
-        pg0 = __builtin_amdgcn_readfirstlane(bt[min(pb + 2 * kt, pe - 1)]);
-        pg1 = __builtin_amdgcn_readfirstlane(bt[min(pb + 2 * kt + 1, pe - 1)]);
-    };
     f32x4 raw[VM][2];
     auto load_raw = [&](int pg0, int pg1) {
 #pragma unroll
@@ -342,7 +373,7 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
             bf16x8 p[3];
             split3_bf16x8(x, p);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) lds[slot][slice][k][f * 64 + lane] = p[k];
+            for (int k = 0; k < 3; ++k) lds(slot, k)[f * 64 + lane] = p[k];
         }
     };
 
@@ -353,16 +384,16 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
         for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
     float m = -INFINITY, lsum = 0.0f;
     const int nsteps = (kt1 - kt0 + KW - 1) / KW;
-    int pg0, pg1, npg0, npg1;
-    tile_pages(kt0 + slice, pg0, pg1);
-    tile_pages(kt0 + KW + slice, npg0, npg1);
+    int pg0, pg1;
+    pages.tile(slice, lane, pg0, pg1);
     load_raw(pg0, pg1);
-    const int grow = a.rows[row0 + (valid ? rloc : 0)];
-    bf16x8 q[D / 16][3];
-    shared_load_q<D>(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h, a.scale_log2, valid, q);
+    SharedQ<D> qx;
+    qx.load(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h);
     store_split(0);
-    load_raw(npg0, npg1);
-    tile_pages(kt0 + 2 * KW + slice, npg0, npg1);
+    bf16x8 q[D / 16][3];
+    qx.split(a.scale_log2, q);
+    pages.tile(KW + slice, lane, pg0, pg1);
+    load_raw(pg0, pg1);
 
     auto v_frags = [&](const bf16x8* plane, bf16x8 (&v)[2][D / 32]) {
         const bf16x4* sv = (const bf16x4*)plane;
@@ -382,7 +413,7 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
         ring_barrier<63>();  // the slot is written (LDS only: the next tile's loads stay in flight)
         const int kt = kt0 + KW * t + slice;
         if (busy && kt < kt1) {
-            const bf16x8(&st)[3][CHUNKS] = lds[t & 1][slice];
+            const bf16x8* st[3] = {lds(t & 1, 0), lds(t & 1, 1), lds(t & 1, 2)};
             const int kbase = ((lane >> 4) & 1) * 2 * (2 * D) + (lane & 15);
             f32x16 s;
 #pragma unroll
@@ -429,100 +460,335 @@ __global__ __launch_bounds__(64 * CW * KW, CW * KW / 4) void shared_prefix_f32_k
         if (t + 1 < nsteps) {
             store_split((t + 1) & 1);  // last read in step t - 1, a barrier ago
             if (t + 2 < nsteps) {
-                load_raw(npg0, npg1);
-                tile_pages(kt0 + KW * (t + 3) + slice, npg0, npg1);
+                pages.tile(KW * (t + 2) + slice, lane, pg0, pg1);
+                load_raw(pg0, pg1);
             }
         }
     }
-    shared_finish<D, CW, KW>(a, o, m, lsum, (float*)&lds[0][0][0][0], slice, wq, lane, kvh, item0, nsplits, valid);
+    shared_finish<D, CW, KW>(a, o, m, lsum, (float*)buf, slice, wq, lane, kvh, item0, nsplits, valid);
 }
 
-// Joins a row's partials.  A wave per (row, q head): lane s takes part s's
-// (m, l) (64 at a time), then every lane its D / 64 dims of every part.  Parts
-// are summed in the order of the row's sources (segments, then its own pages).
-// rec: {row, first source, sources, 0}; src: {first item, parts, first column, 0}.
+// A tail: one wave per kv head of one split of a decode tile, 16 columns = (query,
+// q head of the kv head) pairs of one sequence, its own pages two at a time
+// through a ring of RING page sets in registers (the first four ids in the
+// record); the partial goes out.  Per page pair (lane l, column l % 16, quad
+// l / 16), on v_mfma_f32_16x16x32_bf16: S^T = K Q^T, an online softmax step over
+// 32 keys, O^T += V^T P^T with P^T the lane's own scores.  Q and P (f32 pools: K
+// and V) in three bf16 parts as in the units; bound by the pages.
+template <int D>
+__device__ __forceinline__ f32x4 tail_qk(const PageRegs<uint16_t, D>& pg, const bf16x8* q, int lane) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < D / 32; ++kb)
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pg.k[kb], q[(i * (D / 32) + kb) * 64 + lane], s, 0, 0, 0);
+    return s;
+}
+
+template <int D>
+__device__ __forceinline__ f32x4 tail_qk(const PageRegs<float, D>& pg, const bf16x8* q, int lane) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < D / 32; ++kb) {
+        float kf[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) kf[j] = pg.k[kb][j >> 2][j & 3];
+        bf16x8 k[3];
+        split3_bf16x8(kf, k);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const bf16x8 qi = q[(i * (D / 32) + kb) * 64 + lane];
+#pragma unroll
+            for (int j = 0; j < 3 - i; ++j) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[j], qi, s, 0, 0, 0);
+        }
+    }
+    return s;
+}
+
+template <int D>
+__device__ __forceinline__ void tail_pv(const PageRegs<uint16_t, D>& pa, const PageRegs<uint16_t, D>& pb,
+                                        const bf16x8 (&p)[3], f32x4* o) {
+#pragma unroll
+    for (int vb = 0; vb < D / 32; ++vb) {
+        const bf16x8 v0 = __builtin_shufflevector(pa.v[vb], pb.v[vb], 0, 1, 2, 3, 8, 9, 10, 11);
+        const bf16x8 v1 = __builtin_shufflevector(pa.v[vb], pb.v[vb], 4, 5, 6, 7, 12, 13, 14, 15);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            o[2 * vb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, p[i], o[2 * vb], 0, 0, 0);
+            o[2 * vb + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, p[i], o[2 * vb + 1], 0, 0, 0);
+        }
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void tail_pv(const PageRegs<float, D>& pa, const PageRegs<float, D>& pb,
+                                        const bf16x8 (&p)[3], f32x4* o) {
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) {
+        const f32x4 va = pa.v[db >> 1][db & 1], vb = pb.v[db >> 1][db & 1];
+        const float vf[8] = {va[0], va[1], va[2], va[3], vb[0], vb[1], vb[2], vb[3]};
+        bf16x8 v[3];
+        split3_bf16x8(vf, v);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int j = 0; j < 3 - i; ++j) o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[j], p[i], o[db], 0, 0, 0);
+    }
+}
+
+constexpr size_t tail_lds(int D) { return (size_t)4 * 3 * (D / 32) * 64 * 16; }
+
+template <typename KV, int D, int RING>
+__device__ __forceinline__ void shared_tail(const SharedArgs& a, const int* __restrict__ block_tables, int group,
+                                            bf16x8* buf) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Workgroups go to the 8 XCDs round-robin; on each, wave n of the tails takes
+    // kv head n % kv_heads of every eighth record, so that all of a tail's pages
+    // go through one XCD.
+    const int n = group * 4 + wave;
+    const int kvh = n % a.kv_heads;
+    const int rank = (n / a.kv_heads) * 8 + (blockIdx.x & 7);
+    if (rank >= a.n_tails) return;  // (no barrier in a tail)
+    const int4 r0 = a.rec[3 * rank], r1 = a.rec[3 * rank + 1], r2 = a.rec[3 * rank + 2];
+    const int seq = r0.x, row0 = r0.y, nq = r0.z, page_b = r0.w, page_e = r1.x, foff = r1.z;
+    if (nq == 0) return;  // an empty record past a replayed bucket's items
+    const int item = (int)((unsigned)r1.w & (kAttnSingle - 1));
+    const int c = lane & 15, q4 = lane >> 4;
+    const int qi = c / a.G, g = c - qi * a.G;
+    const bool valid = qi < nq;                  // (16 is a multiple of G)
+    const int jmax = r1.y + (valid ? qi : 0);    // last visible key of the column
+    const KV* pool = (const KV*)a.pool;
+    const int* bt = block_tables + (size_t)seq * a.stride;
+    const size_t kv_tile = (size_t)kPageRows * D;
+    const size_t v_block = (size_t)a.kv_heads * kv_tile;
+    PageRegs<KV, D> ring[RING];
+    auto load_page = [&](PageRegs<KV, D>& r, int page) {
+        const KV* base = pool + (size_t)page * a.page_elems + (size_t)kvh * kv_tile;
+        r.load(base, base + v_block, lane);
+    };
+    // (every slot is loaded: past the end, a page already asked for)
+    auto load_next = [&](PageRegs<KV, D>& r, int p) { load_page(r, bt[min(p, page_e - 1)]); };
+    f32x4 qx[D / 32][2];
+    const float* qp = a.q + (size_t)(row0 + (valid ? qi : 0)) * a.q_cols + (size_t)(kvh * a.G + g) * D + q4 * 8;
+#pragma unroll
+    for (int kb = 0; kb < D / 32; ++kb) {
+        qx[kb][0] = *(const f32x4*)(qp + kb * 32);
+        qx[kb][1] = *(const f32x4*)(qp + kb * 32 + 4);
+    }
+    static_assert(RING % 2 == 0 && RING >= 4 && RING - 2 <= 4, "ring of page pairs; the record holds 4 pages");
+    const int first_pages[4] = {r2.x, r2.y, r2.z, r2.w};
+#pragma unroll
+    for (int r = 0; r < RING - 2; ++r) load_page(ring[r], first_pages[r]);
+    bf16x8* qs = buf + (size_t)wave * 3 * (D / 32) * 64;
+#pragma unroll
+    for (int kb = 0; kb < D / 32; ++kb) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = qx[kb][j >> 2][j & 3] * a.scale_log2;
+        bf16x8 q3[3];
+        split3_bf16x8(x, q3);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) qs[(i * (D / 32) + kb) * 64 + lane] = q3[i];
+    }
+    f32x4 o[D / 16];
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, lsum = 0.0f;
+    auto step = [&](const PageRegs<KV, D>& pa, const PageRegs<KV, D>& pb, int p, bool has_b) {
+        const f32x4 sa = tail_qk<D>(pa, qs, lane);
+        const f32x4 sb = tail_qk<D>(pb, qs, lane);
+        float sc[8], pmax = -INFINITY;
+        const int j0 = p * kPageRows + q4 * 4 - foff;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int ja = j0 + i, jb = ja + kPageRows;
+            sc[i] = ja >= 0 && ja <= jmax ? sa[i] : -INFINITY;
+            sc[4 + i] = has_b && jb <= jmax ? sb[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pmax = fmaxf(pmax, sc[i]);
+        pmax = quad_max(pmax);
+        const float mn = fmaxf(m, pmax);
+        const float mu = mn == -INFINITY ? 0.0f : mn;  // no visible key so far
+        const float alpha = __builtin_amdgcn_exp2f(m - mu);
+        float pr[8], ps = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            pr[i] = __builtin_amdgcn_exp2f(sc[i] - mu);
+            ps += pr[i];
+        }
+        lsum = lsum * alpha + ps;
+        m = mn;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[db][i] *= alpha;
+        bf16x8 p3[3];
+        split3_bf16x8(pr, p3);
+        tail_pv<D>(pa, pb, p3, o);
+    };
+    for (int p = page_b; p < page_e; p += RING) {
+#pragma unroll
+        for (int r = 0; r < RING; r += 2) {
+            const int pp = p + r;
+            if (pp >= page_e) break;
+            load_next(ring[(r + RING - 2) % RING], pp + RING - 2);
+            load_next(ring[(r + RING - 1) % RING], pp + RING - 1);
+            const bool has_b = pp + 1 < page_e;
+            step(ring[r], has_b ? ring[r + 1] : ring[r], pp, has_b);
+        }
+    }
+    lsum += __shfl_xor(lsum, 16, 64);
+    lsum += __shfl_xor(lsum, 32, 64);
+    if (!valid) return;
+    float* out = a.part + (((size_t)item * a.kv_heads + kvh) * 16 + c) * (D + 2);
+    if (q4 == 0) *(float2*)out = make_float2(m, lsum);
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) {
+        float2* x = (float2*)(out + 2 + db * 16 + q4 * 4);
+        x[0] = make_float2(o[db][0], o[db][1]);
+        x[1] = make_float2(o[db][2], o[db][3]);
+    }
+}
+
+// Workgroups in groups of 8 (one per XCD); the unit groups are spread evenly
+// among the tail groups.
+__device__ __forceinline__ bool shared_split(const SharedArgs& a, int& unit_wg, int& tail_group) {
+    const int grp = blockIdx.x >> 3;
+    const unsigned before = (unsigned long long)grp * a.unit_groups / a.groups;
+    const unsigned after = (unsigned long long)(grp + 1) * a.unit_groups / a.groups;
+    unit_wg = (int)before * 8 + (blockIdx.x & 7);
+    tail_group = grp - (int)before;
+    return after > before;
+}
+
+template <int D, int CW, int KW, int STAGES, int RING>
+__global__ __launch_bounds__(256, 2) void shared_attention_kernel(SharedArgs a, const int* __restrict__ block_tables) {
+    constexpr size_t bytes = unit_lds(D, KW, STAGES) > tail_lds(D) ? unit_lds(D, KW, STAGES) : tail_lds(D);
+    __shared__ bf16x8 buf[bytes / 16];
+    int unit_wg, tail_group;
+    if (shared_split(a, unit_wg, tail_group))
+        shared_unit<D, CW, KW, STAGES>(a, block_tables, unit_wg, buf);
+    else
+        shared_tail<uint16_t, D, RING>(a, block_tables, tail_group, buf);
+}
+
+template <int D, int RING>
+__global__ __launch_bounds__(256, 1) void shared_attention_f32_kernel(SharedArgs a, const int* __restrict__ block_tables) {
+    constexpr size_t bytes = unit_f32_lds(D) > tail_lds(D) ? unit_f32_lds(D) : tail_lds(D);
+    __shared__ bf16x8 buf[bytes / 16];
+    int unit_wg, tail_group;
+    if (shared_split(a, unit_wg, tail_group))
+        shared_unit_f32<D>(a, block_tables, unit_wg, buf);
+    else
+        shared_tail<float, D, RING>(a, block_tables, tail_group, buf);
+}
+
+// Joins a row's partials.  A workgroup per (row, q head), 16 lanes per part: lane
+// j of a part holds its dims j D / 16 and on, so 16 parts come in one round trip
+// (4 waves of one part group each: three rounds for 40 parts).  A part group
+// sums the parts p = group mod 16 in order, then the groups meet in LDS, in
+// order: the sums do not depend on timing.
+// rec: {row, first source, sources, parts}; src: {first item, parts, first column, 0}.
 template <int D>
 __global__ __launch_bounds__(256) void shared_merge_kernel(const float* __restrict__ part, const int4* __restrict__ rec,
-                                                           const int4* __restrict__ src, int n_rows, int G, int kv_heads,
-                                                           int q_cols, float* out, uint16_t* out_bf16,
-                                                           size_t lo_offset) {
-    const int lane = threadIdx.x & 63;
+                                                           const int4* __restrict__ src, int G, int kv_heads, int q_cols,
+                                                           float* out, uint16_t* out_bf16, size_t lo_offset) {
+    constexpr int V = D / 16, V2 = V / 2, AHEAD = 2;
+    __shared__ float sm[16], sl[16], so[16][D];
+    const int tid = threadIdx.x, group = tid >> 4, d0 = (tid & 15) * V;
     const int heads = kv_heads * G;
-    const int job = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (job >= n_rows * heads) return;
-    const int ri = job / heads, head = job - ri * heads, kvh = head / G, g = head - kvh * G;
+    const int ri = blockIdx.x / heads, head = blockIdx.x - ri * heads, kvh = head / G, g = head - kvh * G;
     const int4 r = rec[ri];
     if (r.z == 0) return;  // an empty record past a replayed bucket's rows
-    constexpr int V = D / 64;
+    const size_t pstride = (size_t)kv_heads * 16 * (D + 2);
     float M = -INFINITY, L = 0.0f, acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.0f;
-    const size_t pstride = (size_t)kv_heads * 16 * (D + 2);
-    for (int si = 0; si < r.z; ++si) {
-        const int4 s = src[r.y + si];
-        const float* base = part + (((size_t)s.x * kv_heads + kvh) * 16 + s.z + g) * (D + 2);
-        for (int p0 = 0; p0 < s.y; p0 += 64) {
-            const int np = min(64, s.y - p0);
-            float2 ml = make_float2(-INFINITY, 0.0f);
-            if (lane < np) ml = *(const float2*)(base + (size_t)(p0 + lane) * pstride);
-            float mx = ml.x;
+    int si = r.y, start = 0;      // the source holding part p, and its first part
+    int4 s = src[si];
+    for (int p0 = group; p0 < r.w; p0 += 16 * AHEAD) {
+        float2 ml[AHEAD], x[AHEAD][V2];
 #pragma unroll
-            for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-            const float Mn = fmaxf(M, mx);
-            if (Mn == -INFINITY) continue;  // no visible key so far
-            const float keep = exp2f(M - Mn);
-            const float w = exp2f(ml.x - Mn);  // 0 for a part with no visible key
-            float ls = ml.y * w;
+        for (int u = 0; u < AHEAD; ++u) {
+            const int p = p0 + 16 * u;
+            ml[u] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-            for (int off = 32; off > 0; off >>= 1) ls += __shfl_xor(ls, off, 64);
-            L = L * keep + ls;
-            M = Mn;
-#pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] *= keep;
-            const float* pv = base + (size_t)p0 * pstride + 2 + lane * V;
-#pragma unroll 8
-            for (int p = 0; p < np; ++p) {
-                const float wp = __shfl(w, p, 64);
-                if constexpr (V == 2) {
-                    const float2 x = *(const float2*)(pv + (size_t)p * pstride);
-                    acc[0] = fmaf(x.x, wp, acc[0]);
-                    acc[1] = fmaf(x.y, wp, acc[1]);
-                } else {
-                    acc[0] = fmaf(pv[(size_t)p * pstride], wp, acc[0]);
+            for (int j = 0; j < V2; ++j) x[u][j] = make_float2(0.0f, 0.0f);
+            if (p < r.w) {
+                while (p - start >= s.y) {
+                    start += s.y;
+                    s = src[++si];
                 }
+                const float* b =
+                    part + (((size_t)s.x * kv_heads + kvh) * 16 + s.z + g) * (D + 2) + (size_t)(p - start) * pstride;
+                ml[u] = *(const float2*)b;
+#pragma unroll
+                for (int j = 0; j < V2; ++j) x[u][j] = *(const float2*)(b + 2 + d0 + 2 * j);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const float Mn = fmaxf(M, ml[u].x);
+            if (Mn == -INFINITY) continue;  // no visible key so far
+            const float keep = exp2f(M - Mn), w = exp2f(ml[u].x - Mn);
+            M = Mn;
+            L = L * keep + ml[u].y * w;
+#pragma unroll
+            for (int j = 0; j < V2; ++j) {
+                acc[2 * j] = fmaf(x[u][j].x, w, acc[2 * j] * keep);
+                acc[2 * j + 1] = fmaf(x[u][j].y, w, acc[2 * j + 1] * keep);
             }
         }
     }
-    const float inv = 1.0f / L;
-    const int col = head * D + lane * V;
+    if ((tid & 15) == 0) {
+        sm[group] = M;
+        sl[group] = L;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) so[group][d0 + j] = acc[j];
+    __syncthreads();
+    if (tid >= D) return;
+    float mm = sm[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mm = fmaxf(mm, sm[i]);
+    float l = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float w = sm[i] == -INFINITY ? 0.0f : exp2f(sm[i] - mm);
+        l = fmaf(sl[i], w, l);
+        o = fmaf(so[i][tid], w, o);
+    }
+    o /= l;
+    const int col = head * D + tid;
     if (out_bf16) {
-        const size_t o = a_pack_index(r.x, col, q_cols);  // V consecutive columns are one run of the packed operand
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            uint16_t hi, lo;
-            split_bf16(acc[j] * inv, hi, lo);
-            out_bf16[o + j] = hi;
-            if (lo_offset) out_bf16[lo_offset + o + j] = lo;
-        }
+        uint16_t hi, lo;
+        split_bf16(o, hi, lo);
+        const size_t at = a_pack_index(r.x, col, q_cols);
+        out_bf16[at] = hi;
+        if (lo_offset) out_bf16[lo_offset + at] = lo;
     } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) out[(size_t)r.x * q_cols + col + j] = acc[j] * inv;
+        out[(size_t)r.x * q_cols + col] = o;
     }
 }
 
 template <int D>
-static void launch_units(zr_context* ctx, StagedMeta* st, const SharedArgs& a) {
-    const dim3 grid(st->n_sunits * ctx->local_kv_heads);
-    constexpr int KW = D == 64 ? 2 : 1;
-    if (ctx->desc.kv_dtype == ZR_DTYPE_BF16)
-        hipLaunchKernelGGL((shared_prefix_kernel<D, 4, 2, 3>), grid, dim3(512), 0, ctx->stream, a, st->block_tables);
+static void launch_shared(zr_context* ctx, StagedMeta* st, const SharedArgs& a) {
+    const dim3 grid(8 * a.groups), block(256);
+    constexpr int RING = D == 64 ? 6 : 4;
+    if (ctx->desc.kv_dtype == ZR_DTYPE_F32)
+        hipLaunchKernelGGL((shared_attention_f32_kernel<D, 4>), grid, block, 0, ctx->stream, a, st->block_tables);
+    else if (st->unit_cols == 128)
+        hipLaunchKernelGGL((shared_attention_kernel<D, 4, 1, 3, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
+    else if (st->unit_cols == 64)
+        hipLaunchKernelGGL((shared_attention_kernel<D, 2, 2, D == 64 ? 3 : 2, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
     else
-        hipLaunchKernelGGL((shared_prefix_f32_kernel<D, 4, KW>), grid, dim3(256 * KW), 0, ctx->stream, a,
-                           st->block_tables);
+        hipLaunchKernelGGL((shared_attention_kernel<D, 1, 4, 2, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
 }
 
-zr_status launch_shared_prefix(zr_context* ctx, StagedMeta* st, int layer, const float* q) {
-    if (st->n_sunits == 0) return ZR_OK;
+zr_status launch_shared_attention(zr_context* ctx, StagedMeta* st, int layer, const float* q) {
     const size_t esz = ctx->desc.kv_dtype == ZR_DTYPE_BF16 ? 2 : 4;
     SharedArgs a;
     a.q = q;
@@ -530,17 +796,20 @@ zr_status launch_shared_prefix(zr_context* ctx, StagedMeta* st, int layer, const
     a.page_elems = (size_t)2 * ctx->kv_cols * kPageRows;
     a.pool = (const unsigned char*)ctx->kv_pool + (size_t)layer * ctx->n_pages * a.page_elems * esz;
     a.stride = st->stride;
-    a.first_offset = st->first_offset;
     a.units = st->sunits;
     a.rows = st->srows;
+    a.rec = st->attn_rec;
     a.n_units = st->n_sunits;
-    a.G = ctx->q_per_kv;
+    a.n_tails = st->grid_items;
     a.kv_heads = ctx->local_kv_heads;
+    a.unit_groups = (a.n_units * a.kv_heads + 7) / 8;
+    a.groups = a.unit_groups + ((a.n_tails + 7) / 8 * a.kv_heads + 3) / 4;
+    a.G = ctx->q_per_kv;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)ctx->head_dim);
     a.part = ctx->attn_part;
     hipEvent_t ev;
     timing_mark_begin(ctx, kClassAttention, &ev);
-    if (ctx->head_dim == 64) launch_units<64>(ctx, st, a); else launch_units<128>(ctx, st, a);
+    if (ctx->head_dim == 64) launch_shared<64>(ctx, st, a); else launch_shared<128>(ctx, st, a);
     ZR_LAUNCH_CHECK(ctx);
     timing_mark_end(ctx, kClassAttention, ev);
     return ZR_OK;
@@ -549,15 +818,15 @@ zr_status launch_shared_prefix(zr_context* ctx, StagedMeta* st, int layer, const
 zr_status launch_shared_merge(zr_context* ctx, StagedMeta* st, float* out, uint16_t* out_bf16) {
     if (st->n_smerge == 0) return ZR_OK;
     const size_t lo = (ctx->desc.flags & ZR_FLAG_SPLIT_ACTIVATIONS) ? a_plane(st->total_q, ctx->q_cols) : 0;
-    const dim3 grid((st->n_smerge * ctx->local_q_heads + 3) / 4);
+    const dim3 grid(st->n_smerge * ctx->local_q_heads);
     hipEvent_t ev;
     timing_mark_begin(ctx, kClassOther, &ev);
     if (ctx->head_dim == 64)
         hipLaunchKernelGGL((shared_merge_kernel<64>), grid, dim3(256), 0, ctx->stream, ctx->attn_part, st->smerge,
-                           st->ssrc, st->n_smerge, ctx->q_per_kv, ctx->local_kv_heads, ctx->q_cols, out, out_bf16, lo);
+                           st->ssrc, ctx->q_per_kv, ctx->local_kv_heads, ctx->q_cols, out, out_bf16, lo);
     else
         hipLaunchKernelGGL((shared_merge_kernel<128>), grid, dim3(256), 0, ctx->stream, ctx->attn_part, st->smerge,
-                           st->ssrc, st->n_smerge, ctx->q_per_kv, ctx->local_kv_heads, ctx->q_cols, out, out_bf16, lo);
+                           st->ssrc, ctx->q_per_kv, ctx->local_kv_heads, ctx->q_cols, out, out_bf16, lo);
     ZR_LAUNCH_CHECK(ctx);
     timing_mark_end(ctx, kClassOther, ev);
     return ZR_OK;

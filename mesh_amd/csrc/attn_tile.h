@@ -1,11 +1,56 @@
-// Steps on one tile of scores that the attention kernels over 32-key tiles share
-// (v_mfma_f32_32x32x16_bf16: a lane holds 16 scores of one column, lane l ^ 32
-// the other 16).
+// What the attention kernels share: a page's registers, operands in bf16 parts, and
+// steps on one tile of scores (v_mfma_f32_32x32x16_bf16: a lane holds 16 scores of
+// one column, lane l ^ 32 the other 16).
 #pragma once
 
 #include "zr_internal.h"
 
 namespace zr {
+
+// Every page of the pool is read once per launch (one workgroup per kv head
+// and page run), so the loads carry the nontemporal hint: the lines are
+// streamed through L2 with low retention instead of displacing what the other
+// waves on the XCD still read (256-session Llama-3-8B step: attention 9.55-9.78
+// -> 8.81-8.99 ms per step; 32-session TinyLlama step unchanged).
+template <typename KV, int D> struct PageRegs;
+
+// bf16 pool: K fragment per 32 dims = 8 bf16 (16 B); V per 32 dims = 8 bf16
+// (16 B): tokens 4 q4 .. 4 q4 + 3 of dims 32 vb + c, then of 32 vb + 16 + c.
+// Both are one 1 KiB contiguous wave load.
+template <int D> struct PageRegs<uint16_t, D> {
+    bf16x8 k[D / 32];
+    bf16x8 v[D / 32];
+    __device__ inline void load(const uint16_t* kp, const uint16_t* vp, int lane) {
+#pragma unroll
+        for (int kb = 0; kb < D / 32; ++kb)
+            k[kb] = __builtin_nontemporal_load((const bf16x8*)(kp + ((size_t)kb * kWave + lane) * 8));
+#pragma unroll
+        for (int vb = 0; vb < D / 32; ++vb)
+            v[vb] = __builtin_nontemporal_load((const bf16x8*)(vp + ((size_t)vb * kWave + lane) * 8));
+    }
+};
+
+// f32 pool (page_order): the same 8 values per lane and 32 dims, as two
+// 16 B halves that each come from one contiguous 1 KiB wave run (K: dims
+// 8 g + [0, 4) then + [4, 8); V: dim d then d + 16, 4 tokens each).
+template <int D> struct PageRegs<float, D> {
+    f32x4 k[D / 32][2];
+    f32x4 v[D / 32][2];
+    __device__ inline void load(const float* kp, const float* vp, int lane) {
+#pragma unroll
+        for (int kb = 0; kb < D / 32; ++kb) {
+            const f32x4* src = (const f32x4*)(kp + (size_t)kb * kWave * 8) + lane;
+            k[kb][0] = __builtin_nontemporal_load(src);
+            k[kb][1] = __builtin_nontemporal_load(src + kWave);
+        }
+#pragma unroll
+        for (int vb = 0; vb < D / 32; ++vb) {
+            const f32x4* src = (const f32x4*)(vp + (size_t)vb * kWave * 8) + lane;
+            v[vb][0] = __builtin_nontemporal_load(src);
+            v[vb][1] = __builtin_nontemporal_load(src + kWave);
+        }
+    }
+};
 
 // x[0..7] as bf16 hi + lo fragments, two values per v_cvt_pk_bf16_f32 (the
 // same bits as split_bf16)
@@ -98,6 +143,15 @@ __device__ __forceinline__ void prefill_softmax(const f32x16& s, f32x16 (&o)[D /
         pr[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
         lsum += pr[i];
     }
+}
+
+// max over the lanes {l, l^16, l^32, l^48} (the four quads holding one column),
+// with gfx950's VALU lane swaps.
+__device__ inline float quad_max(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 }  // namespace zr

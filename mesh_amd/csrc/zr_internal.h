@@ -322,8 +322,10 @@ struct StagedMeta {
     // sequences that share leading pages (attention_shared.hip)
     int n_segments = 0;       // runs of shared pages
     int n_sunits = 0;         // work units of the shared-prefix launch (per kv head)
-    int n_smerge = 0;         // query rows whose partials shared_merge_kernel joins
-    int shared_seqs = 0, shared_saved = 0;  // sequences in segments; page reads they save per kv head and launch
+    int n_smerge = 0;         // query rows whose partials shared_merge_kernel joins (all that run as decode tiles)
+    int unit_cols = 128;      // columns of a unit: 32, 64 or 128
+    int shared_seqs = 0, shared_rows = 0, shared_saved = 0;  // sequences in segments, their query rows; page reads
+                                                             // saved per kv head and launch
     int grid_items = 0;       // decode attention records the launch covers (n_attn_items, or a bucket's
                               // capacity whose records past n_attn_items are empty)
     int grid_merge = 0;       // merge records the launch covers (likewise)
@@ -352,9 +354,10 @@ struct StagedMeta {
     int4* pblocks = nullptr;    // [n_pblocks] {seq, r0, nrows, pages}, most key tiles first (plain layout:
                                 // {seq, first column, columns, pages}, column = row x q heads per kv head + head)
     int4* psplits = nullptr;    // [n_pblocks] {first key tile, end key tile, item, splits}
-    int4* sunits = nullptr;     // [n_sunits][2] {seq, first row in srows, rows | splits << 16, first page},
+    int4* sunits = nullptr;     // [n_sunits][2] {seq | first row of its first page << 27, first row in srows,
+                                // rows | splits << 16, first page},
                                 // {first key tile, end key tile, partial item, end page}
-    int4* smerge = nullptr;     // [n_smerge] {row, first source, sources, 0}
+    int4* smerge = nullptr;     // [n_smerge] {row, first source, sources, parts}
     int4* ssrc = nullptr;       // partials of a row: {first item, parts, first column of its 16, 0}
     int* srows = nullptr;       // query rows of the units
     // host copies
@@ -434,9 +437,9 @@ zr_status launch_rope_kv_write(zr_context* ctx, StagedMeta* st, int layer, const
 // out_f32 [T, q_cols] or out_bf16 (A operand of the O projection).
 zr_status launch_attention(zr_context* ctx, StagedMeta* st, int layer, const float* q, float* out_f32,
                            uint16_t* out_bf16);
-// The staged segments' partials, and the join of their rows with the partials of
-// the rows' own pages.
-zr_status launch_shared_prefix(zr_context* ctx, StagedMeta* st, int layer, const float* q);
+// Microbatches with shared segments: the partials of the segments and of every
+// decode tile's own pages, and the join of each row's.
+zr_status launch_shared_attention(zr_context* ctx, StagedMeta* st, int layer, const float* q);
 zr_status launch_shared_merge(zr_context* ctx, StagedMeta* st, float* out_f32, uint16_t* out_bf16);
 // Plain-layout pools with head_dim a multiple of 4 (tiles staged in pblocks).
 zr_status launch_attention_plain(zr_context* ctx, StagedMeta* st, int layer, const float* q, float* out_f32,
