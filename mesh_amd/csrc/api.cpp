@@ -153,14 +153,14 @@ static inline size_t align16(size_t x) { return (x + 15) & ~(size_t)15; }
 // Offsets of one staged blob: the host-written inputs and records first, then
 // the arrays the pack stage derives on the device.
 struct BlobLayout {
-    size_t o_qlen, o_kvb, o_fpos, o_foff, o_bt, o_tok, o_arec, o_mrec, o_pblk, o_psplit, o_sunit, o_smrg, o_ssrc, o_srow,
+    size_t o_qlen, o_kvb, o_fpos, o_foff, o_bt, o_tok, o_arec, o_mrec, o_pblk, o_psplit, o_sunit, o_smrg, o_ssrc,
         host_bytes;
     size_t o_cuq, o_cuk, o_pos, o_slot, o_seq, o_last, o_rcs, total_bytes;
 };
 
 // records of the shared-prefix launch and its merge
 struct SharedCounts {
-    int units = 0, merges = 0, sources = 0, rows = 0;
+    int units = 0, merges = 0, sources = 0;
 };
 
 static BlobLayout blob_layout(int S, int stride, int total_q, int n_items, int n_merge, int n_pblocks, int head_dim,
@@ -182,10 +182,9 @@ static BlobLayout blob_layout(int S, int stride, int total_q, int n_items, int n
     b.o_mrec = take(16 * (size_t)std::max(n_merge, 1));
     b.o_pblk = take(16 * (size_t)std::max(n_pblocks, 1));
     b.o_psplit = take(16 * (size_t)std::max(n_pblocks, 1));
-    b.o_sunit = take(32 * (size_t)sh.units);
+    b.o_sunit = take(4 * (size_t)kUnitInts * sh.units);
     b.o_smrg = take(16 * (size_t)sh.merges);
     b.o_ssrc = take(16 * (size_t)sh.sources);
-    b.o_srow = take(4 * (size_t)sh.rows);
     b.host_bytes = off;
     b.o_cuq = take(4 * (S + 1));
     b.o_cuk = take(4 * (S + 1));
@@ -277,6 +276,30 @@ int prefill_tiles_per_split(const int* ktiles, int n, int kv_heads, int slots) {
         if (p < price) best = lo, price = p;
     }
     return best;
+}
+
+// Steps of key tiles per unit of a shared-segment launch: `steps` in all (over
+// units and kv heads), beside `tail_wgs` workgroups of tails that read
+// `tail_bytes`.  A unit costs about 5 us to start and end and 1.7 us a step with
+// another workgroup on its CU, and leaves unit_part bytes of partials, written
+// and read again; HBM gives about 5.9 MB a us.  Of the counts of workgroups worth
+// trying, the one whose launch and merge are estimated shortest.
+static int shared_unit_steps(long steps, int tail_wgs, double tail_bytes, double unit_part) {
+    const double hbm = 5.9e6, start = 5.0, step = 1.7;
+    const double tail_us = tail_bytes / hbm;
+    int best = 1;
+    double price = 1e30;
+    for (const int wgs : {64, 96, 128, 192, 256, 320, 384, 448, 512, 768, 1024}) {
+        const int n = (int)((steps + wgs - 1) / wgs);
+        const double units = (double)(steps + n - 1) / n, us = start + step * n;
+        // slots: a tail's workgroup holds one for its share of the bytes' time
+        const double held = units * us + std::max(tail_us * kSharedSlots * 0.7, tail_wgs * 6.0);
+        const bool again = units + tail_wgs > kSharedSlots;  // a second wave of workgroups ends unevenly
+        const double p = std::max(std::max(tail_us, us), held / kSharedSlots + (again ? 0.3 * us : 0.0)) +
+                         2.0 * units * unit_part / hbm;
+        if (p < price) price = p, best = n;
+    }
+    return std::max(best, 1);
 }
 
 zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta* st, const StageFixed* fixed,
@@ -473,7 +496,6 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     st->h_sunits.clear();
     st->h_smerge.clear();
     st->h_ssrc.clear();
-    st->h_srows.clear();
     st->n_segments = (int)segments.size();
     st->shared_seqs = st->shared_rows = st->shared_saved = 0;
     std::vector<std::vector<int4>> row_src;  // by query row: partials {first item, parts, first column of its 16}
@@ -491,29 +513,42 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
         st->unit_cols = f32_kv || most * G > 64 ? 128 : most * G > 32 ? 64 : 32;
         const int upr = st->unit_cols / G, gpr = 16 / G;  // rows per unit and per 16-column group
         const int slices = 128 / st->unit_cols;           // tiles a unit takes at once
+        long tail_pages = 0;
+        for (int p : tile_pages) tail_pages += p;
         long unit_steps = 0;
         for (const SharedSegment& g : segments)
             unit_steps += (long)((rows_of(g) + upr - 1) / upr) * (((g.end - g.begin + 1) / 2 + slices - 1) / slices);
-        const int unit_tps =
-            slices * (int)std::max<long>(2, (unit_steps * ctx->local_kv_heads + 511) / 512);
+        const int unit_tps = slices * shared_unit_steps(unit_steps * ctx->local_kv_heads,
+                                                        ((st->n_attn_items + 7) / 8 * ctx->local_kv_heads + 3) / 4 * 8,
+                                                        (double)tail_pages * ctx->page_bytes, 128 * (ctx->head_dim + 2) * 4.0 / slices);
         for (const SharedSegment& g : segments) {
-            const int row0 = (int)st->h_srows.size();
+            std::vector<int> rows;
             for (int s : g.members)
-                for (int r = cu_rows[s]; r < cu_rows[s + 1]; ++r) st->h_srows.push_back(r);
-            const int rows = (int)st->h_srows.size() - row0;
+                for (int r = cu_rows[s]; r < cu_rows[s + 1]; ++r) rows.push_back(r);
+            const int nr = (int)rows.size();
             const int nt = (g.end - g.begin + 1) / 2, ns = (nt + unit_tps - 1) / unit_tps;
-            const int groups = (rows + gpr - 1) / gpr;
+            const int* bt = mb->block_tables + (size_t)g.seq * stride;
             for (int sp = 0; sp < ns; ++sp)  // the units of a run of tiles side by side: they read the same pages
-                for (int r = 0; r < rows; r += upr) {
-                    const int n = std::min(upr, rows - r);
-                    const unsigned foff = g.begin == 0 ? mb->first_offset[g.seq] : 0;
-                    st->h_sunits.push_back(make_int4((int)(g.seq | foff << 27), row0 + r, n | ns << 16, g.begin));
-                    st->h_sunits.push_back(make_int4((int)((long)sp * nt / ns), (int)((long)(sp + 1) * nt / ns),
-                                                     next_item + (r / gpr) * ns + sp, g.end));
+                for (int r = 0; r < nr; r += upr) {
+                    const int n = std::min(upr, nr - r);
+                    const int kt0 = (int)((long)sp * nt / ns), kt1 = (int)((long)(sp + 1) * nt / ns);
+                    const size_t at = st->h_sunits.size();
+                    st->h_sunits.resize(at + kUnitInts, 0);
+                    int* u = st->h_sunits.data() + at;
+                    u[0] = g.seq;
+                    u[1] = g.begin == 0 ? mb->first_offset[g.seq] : 0;
+                    u[2] = n | ns << 16;
+                    u[3] = g.begin;
+                    u[4] = kt0;
+                    u[5] = kt1;
+                    u[6] = next_item + (r / gpr) * ns + sp;
+                    u[7] = g.end;
+                    for (int i = 0; i < 64; ++i) u[kUnitPages + i] = bt[std::min(g.begin + 2 * kt0 + i, g.end - 1)];
+                    for (int i = 0; i < 128; ++i) u[kUnitRows + i] = rows[r + std::min(i, n - 1)];
                 }
-            for (int r = 0; r < rows; ++r)
-                row_src[st->h_srows[row0 + r]].push_back(make_int4(next_item + (r / gpr) * ns, ns, (r % gpr) * G, 0));
-            next_item += groups * ns;
+            for (int r = 0; r < nr; ++r)
+                row_src[rows[r]].push_back(make_int4(next_item + (r / gpr) * ns, ns, (r % gpr) * G, 0));
+            next_item += (nr + gpr - 1) / gpr * ns;
             st->shared_saved += ((int)g.members.size() - 1) * (g.end - g.begin);
         }
         // ... and the partials of the rows' own pages
@@ -534,8 +569,12 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
             }
         }
     }
-    st->n_sunits = (int)st->h_sunits.size() / 2;
+    st->n_sunits = (int)st->h_sunits.size() / kUnitInts;
     st->n_smerge = (int)st->h_smerge.size();
+    // 16 parts come in one round trip of one wave
+    int parts = 0;
+    for (const int4& r : st->h_smerge) parts = std::max(parts, r.w);
+    st->merge_wide = parts > 16 && (long)st->n_smerge * ctx->local_q_heads <= 4096;
     st->n_part_items = next_item;
     // dispatch order: longest items first, so the short ones fill the tail
     st->h_order.resize(st->n_attn_items);
@@ -645,7 +684,6 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     sh.units = st->n_sunits;
     sh.merges = st->n_smerge;
     sh.sources = (int)st->h_ssrc.size();
-    sh.rows = (int)st->h_srows.size();
     const BlobLayout L = blob_layout(S, blob_stride, total_q, st->grid_items, st->grid_merge, st->n_pblocks,
                                      ctx->head_dim, sh);
     const size_t host_bytes = L.host_bytes, total_bytes = L.total_bytes;
@@ -693,16 +731,14 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     if (st->n_pblocks) memcpy(hb + L.o_pblk, st->h_pblocks.data(), 16 * (size_t)st->n_pblocks);
     if (st->n_pblocks) memcpy(hb + L.o_psplit, st->h_psplits.data(), 16 * (size_t)st->n_pblocks);
     if (st->n_sunits) {
-        memcpy(hb + L.o_sunit, st->h_sunits.data(), 16 * st->h_sunits.size());
+        memcpy(hb + L.o_sunit, st->h_sunits.data(), 4 * st->h_sunits.size());
         memcpy(hb + L.o_smrg, st->h_smerge.data(), 16 * st->h_smerge.size());
         memcpy(hb + L.o_ssrc, st->h_ssrc.data(), 16 * st->h_ssrc.size());
-        memcpy(hb + L.o_srow, st->h_srows.data(), 4 * st->h_srows.size());
     }
     unsigned char* db = (unsigned char*)st->dev;
-    st->sunits = (int4*)(db + L.o_sunit);
+    st->sunits = (int*)(db + L.o_sunit);
     st->smerge = (int4*)(db + L.o_smrg);
     st->ssrc = (int4*)(db + L.o_ssrc);
-    st->srows = (int*)(db + L.o_srow);
     st->q_len = (int*)(db + L.o_qlen);
     st->kv_before = (int*)(db + L.o_kvb);
     st->first_pos = (int*)(db + L.o_fpos);

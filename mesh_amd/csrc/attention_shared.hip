@@ -26,13 +26,10 @@ struct SharedArgs {
     const void* pool;     // layer base of the pool
     size_t page_elems;
     int stride;           // block table row stride (the table is a kernel argument)
-    const int4* units;    // two records per work unit: {seq | first row of its first page << 27, first of its rows in
-                          // `rows`, rows | splits << 16, first page}, {first key tile, end key tile, partial item,
-                          // end page}
-    const int* rows;      // query rows of the microbatch
+    const int* units;     // kUnitInts per work unit (zr_internal.h)
     const int4* rec;      // three records per tail, longest first (AttnArgs::rec)
     int n_units, n_tails;
-    int unit_groups, groups;  // of 8 workgroups: those of units, all
+    int unit_groups, unit_span;  // groups of 8 workgroups: those of units, and the first ones they are spread over
     int G, kv_heads;
     float scale_log2;     // log2(e) / sqrt(d)
     float* part;          // [items][kv_heads][16][D + 2]
@@ -61,8 +58,9 @@ template <int D> struct SharedQ {
 };
 
 // A unit's page ids, 64 at a time, one per lane: a tile's two come by lane reads,
-// so that no table load stands before its copies.  Tiles are asked for in order;
-// one past the segment's end repeats its last page.
+// so that no table load stands before its copies.  The first 64 lie in the unit's
+// record.  Tiles are asked for in order; one past the segment's end repeats its
+// last page.
 struct SharedPages {
     const int* bt;   // the sequence's table from the unit's first page on
     int last;        // last page of the segment, counted from there
@@ -186,27 +184,28 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const int* __re
     const int rank = __builtin_amdgcn_readfirstlane(wg / a.kv_heads);
     const int kvh = wg - rank * a.kv_heads;
     if (rank >= a.n_units) return;
-    const int4 u0 = a.units[2 * rank], u1 = a.units[2 * rank + 1];
-    const int seq = __builtin_amdgcn_readfirstlane(u0.x) & 0x7ffffff, row0 = __builtin_amdgcn_readfirstlane(u0.y);
+    // everything the copies and the Q loads need comes in one round trip
+    const int* unit = a.units + (size_t)rank * kUnitInts;
+    const int4 u0 = ((const int4*)unit)[0], u1 = ((const int4*)unit)[1];
+    const int ids = unit[kUnitPages + lane];
+    const int c = wq * 32 + (lane & 31);
+    const int rloc = c / a.G, g = c - rloc * a.G;
+    const int grow = unit[kUnitRows + rloc];  // (columns past the unit's rows compute its last row, unused)
+    const int seq = __builtin_amdgcn_readfirstlane(u0.x), foff = __builtin_amdgcn_readfirstlane(u0.y);
     const int nrows = __builtin_amdgcn_readfirstlane(u0.z & 0xffff), nsplits = __builtin_amdgcn_readfirstlane(u0.z >> 16);
     const int pb = __builtin_amdgcn_readfirstlane(u0.w), pe = __builtin_amdgcn_readfirstlane(u1.w);
     const int kt0 = __builtin_amdgcn_readfirstlane(u1.x), kt1 = __builtin_amdgcn_readfirstlane(u1.y);
     const int item0 = __builtin_amdgcn_readfirstlane(u1.z);
     if (nrows == 0) return;  // an empty record past a replayed bucket's units
     const int h = lane >> 5;
-    const int c = wq * 32 + (lane & 31);
-    const int rloc = c / a.G, g = c - rloc * a.G;
     const bool valid = rloc < nrows;
     const bool busy = wq * 32 < nrows * a.G;  // the wave has a column
-    // keys of the segment's first page before the window, and of its last tile past its end
-    const int foff = __builtin_amdgcn_readfirstlane((unsigned)u0.x >> 27);
+    // (keys before the window lie in the segment's first page, before row foff; those past its end in its last tile)
     const int jlast = (pe - pb) * kPageRows - 1;
 
     const uint16_t* pool = (const uint16_t*)a.pool;
     const int p0 = pb + 2 * kt0;  // the unit's first page
-    SharedPages pages{block_tables + (size_t)seq * a.stride + p0, pe - 1 - p0, 0, 0};
-    pages.fetch(lane);
-    const int grow = a.rows[row0 + (valid ? rloc : 0)];  // (columns past the unit's rows compute its first row, unused)
+    SharedPages pages{block_tables + (size_t)seq * a.stride + p0, pe - 1 - p0, 0, ids};
     const size_t kv_tile = (size_t)kPageRows * D;
     const size_t v_block = (size_t)a.kv_heads * kv_tile;
     const uint32_t page_bytes = (uint32_t)(a.page_elems * 2);
@@ -330,25 +329,26 @@ __device__ __forceinline__ void shared_unit_f32(const SharedArgs& a, const int* 
     const int rank = __builtin_amdgcn_readfirstlane(wg / a.kv_heads);
     const int kvh = wg - rank * a.kv_heads;
     if (rank >= a.n_units) return;
-    const int4 u0 = a.units[2 * rank], u1 = a.units[2 * rank + 1];
-    const int seq = __builtin_amdgcn_readfirstlane(u0.x) & 0x7ffffff, row0 = __builtin_amdgcn_readfirstlane(u0.y);
+    // everything the copies and the Q loads need comes in one round trip
+    const int* unit = a.units + (size_t)rank * kUnitInts;
+    const int4 u0 = ((const int4*)unit)[0], u1 = ((const int4*)unit)[1];
+    const int ids = unit[kUnitPages + lane];
+    const int c = wq * 32 + (lane & 31);
+    const int rloc = c / a.G, g = c - rloc * a.G;
+    const int grow = unit[kUnitRows + rloc];  // (columns past the unit's rows compute its last row, unused)
+    const int seq = __builtin_amdgcn_readfirstlane(u0.x), foff = __builtin_amdgcn_readfirstlane(u0.y);
     const int nrows = __builtin_amdgcn_readfirstlane(u0.z & 0xffff), nsplits = __builtin_amdgcn_readfirstlane(u0.z >> 16);
     const int pb = __builtin_amdgcn_readfirstlane(u0.w), pe = __builtin_amdgcn_readfirstlane(u1.w);
     const int kt0 = __builtin_amdgcn_readfirstlane(u1.x), kt1 = __builtin_amdgcn_readfirstlane(u1.y);
     const int item0 = __builtin_amdgcn_readfirstlane(u1.z);
     if (nrows == 0) return;
     const int h = lane >> 5;
-    const int c = wq * 32 + (lane & 31);
-    const int rloc = c / a.G, g = c - rloc * a.G;
     const bool valid = rloc < nrows;
     const bool busy = wq * 32 < nrows * a.G;
-    const int foff = __builtin_amdgcn_readfirstlane((unsigned)u0.x >> 27);
     const int jlast = (pe - pb) * kPageRows - 1;
 
     const int p0 = pb + 2 * kt0;
-    SharedPages pages{block_tables + (size_t)seq * a.stride + p0, pe - 1 - p0, 0, 0};
-    pages.fetch(lane);
-    const int grow = a.rows[row0 + (valid ? rloc : 0)];
+    SharedPages pages{block_tables + (size_t)seq * a.stride + p0, pe - 1 - p0, 0, ids};
     const size_t kv_tile = (size_t)kPageRows * D;
     const size_t v_block = (size_t)a.kv_heads * kv_tile;
     const float* pool = (const float*)a.pool + (size_t)kvh * kv_tile + 4 * lane;
@@ -654,13 +654,13 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& a, const int* __re
 }
 
 // Workgroups in groups of 8 (one per XCD); the unit groups are spread evenly
-// among the tail groups.
+// over the first unit_span groups.
 __device__ __forceinline__ bool shared_split(const SharedArgs& a, int& unit_wg, int& tail_group) {
-    const int grp = blockIdx.x >> 3;
-    const unsigned before = (unsigned long long)grp * a.unit_groups / a.groups;
-    const unsigned after = (unsigned long long)(grp + 1) * a.unit_groups / a.groups;
+    const unsigned grp = blockIdx.x >> 3, ug = a.unit_groups, span = a.unit_span;
+    const unsigned before = grp < span ? grp * ug / span : ug;
+    const unsigned after = grp + 1 < span ? (grp + 1) * ug / span : ug;
     unit_wg = (int)before * 8 + (blockIdx.x & 7);
-    tail_group = grp - (int)before;
+    tail_group = (int)(grp - before);
     return after > before;
 }
 
@@ -686,34 +686,38 @@ __global__ __launch_bounds__(256, 1) void shared_attention_f32_kernel(SharedArgs
         shared_tail<float, D, RING>(a, block_tables, tail_group, buf);
 }
 
-// Joins a row's partials.  A workgroup per (row, q head), 16 lanes per part: lane
-// j of a part holds its dims j D / 16 and on, so 16 parts come in one round trip
-// (4 waves of one part group each: three rounds for 40 parts).  A part group
-// sums the parts p = group mod 16 in order, then the groups meet in LDS, in
-// order: the sums do not depend on timing.
+// Joins a row's partials.  16 lanes per part: lane j of a part holds its dims
+// j D / 16 and on.  W waves take a (row, q head), so that 4 W parts come at once
+// (AHEAD of those in flight): one wave where rows are many or their parts few,
+// four where a long prefix left many parts to few rows.  A part group sums its
+// parts p = group mod 4 W in order, then the groups meet in order: the sums do
+// not depend on timing.
 // rec: {row, first source, sources, parts}; src: {first item, parts, first column, 0}.
-template <int D>
+template <int D, int W>
 __global__ __launch_bounds__(256) void shared_merge_kernel(const float* __restrict__ part, const int4* __restrict__ rec,
-                                                           const int4* __restrict__ src, int G, int kv_heads, int q_cols,
-                                                           float* out, uint16_t* out_bf16, size_t lo_offset) {
-    constexpr int V = D / 16, V2 = V / 2, AHEAD = 2;
-    __shared__ float sm[16], sl[16], so[16][D];
-    const int tid = threadIdx.x, group = tid >> 4, d0 = (tid & 15) * V;
+                                                           const int4* __restrict__ src, int jobs, int G, int kv_heads,
+                                                           int q_cols, float* out, uint16_t* out_bf16,
+                                                           size_t lo_offset) {
+    constexpr int V = D / 16, V2 = V / 2, GROUPS = 4 * W, AHEAD = W == 1 ? 4 : 2;
+    __shared__ float sm[4][4], sl[4][4], so[4][4][D];  // [wave][group of the wave]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sub = lane >> 4, d0 = (lane & 15) * V;
+    const int job = blockIdx.x * (4 / W) + (W == 1 ? wave : 0);
+    const int group = W == 1 ? sub : wave * 4 + sub;
     const int heads = kv_heads * G;
-    const int ri = blockIdx.x / heads, head = blockIdx.x - ri * heads, kvh = head / G, g = head - kvh * G;
-    const int4 r = rec[ri];
-    if (r.z == 0) return;  // an empty record past a replayed bucket's rows
+    const int ri = job / heads, head = job - ri * heads, kvh = head / G, g = head - kvh * G;
+    const int4 r = job < jobs ? rec[ri] : make_int4(0, 0, 0, 0);  // (empty too: past a replayed bucket's rows)
     const size_t pstride = (size_t)kv_heads * 16 * (D + 2);
     float M = -INFINITY, L = 0.0f, acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.0f;
     int si = r.y, start = 0;      // the source holding part p, and its first part
-    int4 s = src[si];
-    for (int p0 = group; p0 < r.w; p0 += 16 * AHEAD) {
+    int4 s = r.z > 0 ? src[si] : make_int4(0, 0, 0, 0);
+    for (int p0 = group; p0 < r.w; p0 += GROUPS * AHEAD) {
         float2 ml[AHEAD], x[AHEAD][V2];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const int p = p0 + 16 * u;
+            const int p = p0 + GROUPS * u;
             ml[u] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
             for (int j = 0; j < V2; ++j) x[u][j] = make_float2(0.0f, 0.0f);
@@ -743,40 +747,45 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const float* __restri
             }
         }
     }
-    if ((tid & 15) == 0) {
-        sm[group] = M;
-        sl[group] = L;
+    if ((lane & 15) == 0) {
+        sm[wave][sub] = M;
+        sl[wave][sub] = L;
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) so[group][d0 + j] = acc[j];
+    for (int j = 0; j < V; ++j) so[wave][sub][d0 + j] = acc[j];
     __syncthreads();
-    if (tid >= D) return;
-    float mm = sm[0];
+    // (W == 1: each wave its own job; W == 4: the workgroup's D threads the one)
+    const int nt = W == 1 ? 64 : 256, at = W == 1 ? lane : tid, w0 = W == 1 ? wave : 0;
+    if (r.z == 0) return;
+    float mm = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mm = fmaxf(mm, sm[i]);
-    float l = 0.0f, o = 0.0f;
+    for (int i = 0; i < GROUPS; ++i) mm = fmaxf(mm, sm[w0 + i / 4][i & 3]);
+    for (int d = at; d < D; d += nt) {
+        float l = 0.0f, o = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float w = sm[i] == -INFINITY ? 0.0f : exp2f(sm[i] - mm);
-        l = fmaf(sl[i], w, l);
-        o = fmaf(so[i][tid], w, o);
-    }
-    o /= l;
-    const int col = head * D + tid;
-    if (out_bf16) {
-        uint16_t hi, lo;
-        split_bf16(o, hi, lo);
-        const size_t at = a_pack_index(r.x, col, q_cols);
-        out_bf16[at] = hi;
-        if (lo_offset) out_bf16[lo_offset + at] = lo;
-    } else {
-        out[(size_t)r.x * q_cols + col] = o;
+        for (int i = 0; i < GROUPS; ++i) {
+            const float mi = sm[w0 + i / 4][i & 3];
+            const float w = mi == -INFINITY ? 0.0f : exp2f(mi - mm);
+            l = fmaf(sl[w0 + i / 4][i & 3], w, l);
+            o = fmaf(so[w0 + i / 4][i & 3][d], w, o);
+        }
+        o /= l;
+        const int col = head * D + d;
+        if (out_bf16) {
+            uint16_t hi, lo;
+            split_bf16(o, hi, lo);
+            const size_t idx = a_pack_index(r.x, col, q_cols);
+            out_bf16[idx] = hi;
+            if (lo_offset) out_bf16[lo_offset + idx] = lo;
+        } else {
+            out[(size_t)r.x * q_cols + col] = o;
+        }
     }
 }
 
 template <int D>
-static void launch_shared(zr_context* ctx, StagedMeta* st, const SharedArgs& a) {
-    const dim3 grid(8 * a.groups), block(256);
+static void launch_shared(zr_context* ctx, StagedMeta* st, const SharedArgs& a, int groups) {
+    const dim3 grid(8 * groups), block(256);
     constexpr int RING = D == 64 ? 6 : 4;
     if (ctx->desc.kv_dtype == ZR_DTYPE_F32)
         hipLaunchKernelGGL((shared_attention_f32_kernel<D, 4>), grid, block, 0, ctx->stream, a, st->block_tables);
@@ -797,19 +806,20 @@ zr_status launch_shared_attention(zr_context* ctx, StagedMeta* st, int layer, co
     a.pool = (const unsigned char*)ctx->kv_pool + (size_t)layer * ctx->n_pages * a.page_elems * esz;
     a.stride = st->stride;
     a.units = st->sunits;
-    a.rows = st->srows;
     a.rec = st->attn_rec;
     a.n_units = st->n_sunits;
     a.n_tails = st->grid_items;
     a.kv_heads = ctx->local_kv_heads;
     a.unit_groups = (a.n_units * a.kv_heads + 7) / 8;
-    a.groups = a.unit_groups + ((a.n_tails + 7) / 8 * a.kv_heads + 3) / 4;
+    const int groups = a.unit_groups + ((a.n_tails + 7) / 8 * a.kv_heads + 3) / 4;
+    // units run longest: all of them among the first workgroups to be resident
+    a.unit_span = std::min(groups, std::max(a.unit_groups, kSharedSlots / 8));
     a.G = ctx->q_per_kv;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)ctx->head_dim);
     a.part = ctx->attn_part;
     hipEvent_t ev;
     timing_mark_begin(ctx, kClassAttention, &ev);
-    if (ctx->head_dim == 64) launch_shared<64>(ctx, st, a); else launch_shared<128>(ctx, st, a);
+    if (ctx->head_dim == 64) launch_shared<64>(ctx, st, a, groups); else launch_shared<128>(ctx, st, a, groups);
     ZR_LAUNCH_CHECK(ctx);
     timing_mark_end(ctx, kClassAttention, ev);
     return ZR_OK;
@@ -818,15 +828,20 @@ zr_status launch_shared_attention(zr_context* ctx, StagedMeta* st, int layer, co
 zr_status launch_shared_merge(zr_context* ctx, StagedMeta* st, float* out, uint16_t* out_bf16) {
     if (st->n_smerge == 0) return ZR_OK;
     const size_t lo = (ctx->desc.flags & ZR_FLAG_SPLIT_ACTIVATIONS) ? a_plane(st->total_q, ctx->q_cols) : 0;
-    const dim3 grid(st->n_smerge * ctx->local_q_heads);
+    const int jobs = st->n_smerge * ctx->local_q_heads;
+    const bool wide = st->merge_wide;
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(wide ? jobs : (jobs + 3) / 4), dim3(256), 0, ctx->stream, ctx->attn_part,
+                           st->smerge, st->ssrc, jobs, ctx->q_per_kv, ctx->local_kv_heads, ctx->q_cols, out, out_bf16,
+                           lo);
+    };
     hipEvent_t ev;
     timing_mark_begin(ctx, kClassOther, &ev);
-    if (ctx->head_dim == 64)
-        hipLaunchKernelGGL((shared_merge_kernel<64>), grid, dim3(256), 0, ctx->stream, ctx->attn_part, st->smerge,
-                           st->ssrc, ctx->q_per_kv, ctx->local_kv_heads, ctx->q_cols, out, out_bf16, lo);
-    else
-        hipLaunchKernelGGL((shared_merge_kernel<128>), grid, dim3(256), 0, ctx->stream, ctx->attn_part, st->smerge,
-                           st->ssrc, ctx->q_per_kv, ctx->local_kv_heads, ctx->q_cols, out, out_bf16, lo);
+    if (ctx->head_dim == 64) {
+        if (wide) launch(shared_merge_kernel<64, 4>); else launch(shared_merge_kernel<64, 1>);
+    } else {
+        if (wide) launch(shared_merge_kernel<128, 4>); else launch(shared_merge_kernel<128, 1>);
+    }
     ZR_LAUNCH_CHECK(ctx);
     timing_mark_end(ctx, kClassOther, ev);
     return ZR_OK;

@@ -324,6 +324,7 @@ struct StagedMeta {
     int n_sunits = 0;         // work units of the shared-prefix launch (per kv head)
     int n_smerge = 0;         // query rows whose partials shared_merge_kernel joins (all that run as decode tiles)
     int unit_cols = 128;      // columns of a unit: 32, 64 or 128
+    bool merge_wide = false;  // four waves per (row, q head) in the merge
     int shared_seqs = 0, shared_rows = 0, shared_saved = 0;  // sequences in segments, their query rows; page reads
                                                              // saved per kv head and launch
     int grid_items = 0;       // decode attention records the launch covers (n_attn_items, or a bucket's
@@ -354,15 +355,12 @@ struct StagedMeta {
     int4* pblocks = nullptr;    // [n_pblocks] {seq, r0, nrows, pages}, most key tiles first (plain layout:
                                 // {seq, first column, columns, pages}, column = row x q heads per kv head + head)
     int4* psplits = nullptr;    // [n_pblocks] {first key tile, end key tile, item, splits}
-    int4* sunits = nullptr;     // [n_sunits][2] {seq | first row of its first page << 27, first row in srows,
-                                // rows | splits << 16, first page},
-                                // {first key tile, end key tile, partial item, end page}
+    int* sunits = nullptr;      // [n_sunits][kUnitInts]
     int4* smerge = nullptr;     // [n_smerge] {row, first source, sources, parts}
     int4* ssrc = nullptr;       // partials of a row: {first item, parts, first column of its 16, 0}
-    int* srows = nullptr;       // query rows of the units
     // host copies
-    std::vector<int4> h_sunits, h_smerge, h_ssrc;
-    std::vector<int> h_srows;
+    std::vector<int4> h_smerge, h_ssrc;
+    std::vector<int> h_sunits;
     std::vector<int> h_q_len, h_kv_before, h_first_pos, h_first_offset, h_block_tables;
     std::vector<int4> h_items, h_tiles, h_pblocks, h_psplits;
     std::vector<int> h_merge, h_order;
@@ -370,6 +368,12 @@ struct StagedMeta {
     std::vector<uint32_t> h_tokens;
     std::vector<unsigned char> h_blob;
 };
+
+// A work unit of the shared segments' launch: {seq, first_offset where the unit's segment begins the window (else 0),
+// rows | splits << 16, first page of the segment}, {first key tile, end key tile, partial item, end page}, the unit's
+// first 64 pages (the last one repeated), its query rows (likewise), up to 128.
+constexpr int kUnitPages = 8, kUnitRows = 72, kUnitInts = 200;
+constexpr int kSharedSlots = 512;  // resident workgroups of that launch: two per CU
 
 // A run of pages that the block tables of `members` all name at [begin, end).
 struct SharedSegment {
