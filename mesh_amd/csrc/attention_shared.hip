@@ -13,8 +13,8 @@
 // (tails) and leaves partials; shared_merge_kernel joins those of a row.
 //
 // A unit is bound by the MFMAs (each page serves up to 128 columns), a tail by
-// its pages, so the two kinds of workgroup alternate in dispatch order and run
-// side by side on a CU: two of 4 waves each.
+// its pages; the two kinds of workgroup run side by side on a CU, two of 4 waves
+// each.
 #include "attn_tile.h"
 #include "zr_internal.h"
 
@@ -29,7 +29,7 @@ struct SharedArgs {
     const int* units;     // kUnitInts per work unit (zr_internal.h)
     const int4* rec;      // three records per tail, longest first (AttnArgs::rec)
     int n_units, n_tails;
-    int unit_groups, unit_span;  // groups of 8 workgroups: those of units, and the first ones they are spread over
+    int unit_groups;      // of 8 workgroups
     int G, kv_heads;
     float scale_log2;     // log2(e) / sqrt(d)
     float* part;          // [items][kv_heads][16][D + 2]
@@ -568,8 +568,16 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& a, const int* __re
         const KV* base = pool + (size_t)page * a.page_elems + (size_t)kvh * kv_tile;
         r.load(base, base + v_block, lane);
     };
-    // (every slot is loaded: past the end, a page already asked for)
-    auto load_next = [&](PageRegs<KV, D>& r, int p) { load_page(r, bt[min(p, page_e - 1)]); };
+    // the ids of 64 pages at a time, one per lane, so that no table load stands
+    // before a page's (past the split's end: its last page again)
+    int base = page_b, ids = bt[min(page_b + lane, page_e - 1)];
+    auto load_next = [&](PageRegs<KV, D>& r, int p) {
+        if (p >= base + 64) {
+            base += 64;
+            ids = bt[min(base + lane, page_e - 1)];
+        }
+        load_page(r, __builtin_amdgcn_readlane(ids, p - base));
+    };
     f32x4 qx[D / 32][2];
     const float* qp = a.q + (size_t)(row0 + (valid ? qi : 0)) * a.q_cols + (size_t)(kvh * a.G + g) * D + q4 * 8;
 #pragma unroll
@@ -653,15 +661,13 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& a, const int* __re
     }
 }
 
-// Workgroups in groups of 8 (one per XCD); the unit groups are spread evenly
-// over the first unit_span groups.
+// Units first: they run longest, and as many of them as CUs get one each (in turn
+// with the tails, two units shared one CU and two tails another).  Tails go
+// in groups of 8 workgroups, one per XCD.
 __device__ __forceinline__ bool shared_split(const SharedArgs& a, int& unit_wg, int& tail_group) {
-    const unsigned grp = blockIdx.x >> 3, ug = a.unit_groups, span = a.unit_span;
-    const unsigned before = grp < span ? grp * ug / span : ug;
-    const unsigned after = grp + 1 < span ? (grp + 1) * ug / span : ug;
-    unit_wg = (int)before * 8 + (blockIdx.x & 7);
-    tail_group = (int)(grp - before);
-    return after > before;
+    unit_wg = blockIdx.x;
+    tail_group = (int)(blockIdx.x >> 3) - a.unit_groups;
+    return tail_group < 0;
 }
 
 template <int D, int CW, int KW, int STAGES, int RING>
@@ -812,8 +818,6 @@ zr_status launch_shared_attention(zr_context* ctx, StagedMeta* st, int layer, co
     a.kv_heads = ctx->local_kv_heads;
     a.unit_groups = (a.n_units * a.kv_heads + 7) / 8;
     const int groups = a.unit_groups + ((a.n_tails + 7) / 8 * a.kv_heads + 3) / 4;
-    // units run longest: all of them among the first workgroups to be resident
-    a.unit_span = std::min(groups, std::max(a.unit_groups, kSharedSlots / 8));
     a.G = ctx->q_per_kv;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)ctx->head_dim);
     a.part = ctx->attn_part;
