@@ -279,27 +279,23 @@ int prefill_tiles_per_split(const int* ktiles, int n, int kv_heads, int slots) {
 }
 
 // Steps of key tiles per unit of a shared-segment launch: `steps` in all (over
-// units and kv heads), beside `tail_wgs` workgroups of tails that read
-// `tail_bytes`.  A unit costs about 5 us to start and end and 1.7 us a step with
-// another workgroup on its CU, and leaves unit_part bytes of partials, written
-// and read again; HBM gives about 5.9 MB a us.  Of the counts of workgroups worth
-// trying, the one whose launch and merge are estimated shortest.
-static int shared_unit_steps(long steps, int tail_wgs, double tail_bytes, double unit_part) {
-    const double hbm = 5.9e6, start = 5.0, step = 1.7;
-    const double tail_us = tail_bytes / hbm;
+// units and kv heads), beside tails that read `tail_bytes`.  A unit costs about
+// 8 us to start and end, a step 1.15 us (1.6 with another unit on the CU), HBM
+// gives about 5.9 MB a us, and every unit more costs the launch and its merge about
+// 0.1 us (its start, its partials).  Of the counts worth trying, the one whose
+// estimate is shortest (us a pass with 96 / 128 / 192 / 256 / 512 units: 16 forks on
+// 8000 rows 12.1 / 11.6 / 11.7 / 14.0 / 17.5, 48 x 5 rows on 4011, 16 / 4 heads,
+// 52 / 45 / 39 / 44 / 51, 256 behind 4 prompts of 2040 95 / 95 / 97 / 105 / 122).
+static int shared_unit_steps(long steps, double tail_bytes) {
     int best = 1;
     double price = 1e30;
-    for (const int wgs : {64, 96, 128, 192, 256, 320, 384, 448, 512, 768, 1024}) {
-        const int n = (int)((steps + wgs - 1) / wgs);
-        const double units = (double)(steps + n - 1) / n, us = start + step * n;
-        // slots: a tail's workgroup holds one for its share of the bytes' time
-        const double held = units * us + std::max(tail_us * kSharedSlots * 0.7, tail_wgs * 6.0);
-        const bool again = units + tail_wgs > kSharedSlots;  // a second wave of workgroups ends unevenly
-        const double p = std::max(std::max(tail_us, us), held / kSharedSlots + (again ? 0.3 * us : 0.0)) +
-                         2.0 * units * unit_part / hbm;
+    for (const int wgs : {16, 32, 64, 96, 128, 192, 256, 384, 512, 1024}) {
+        const int n = (int)std::max<long>(1, (steps + wgs - 1) / wgs);
+        const long units = (steps + n - 1) / n;
+        const double p = std::max(tail_bytes / 5.9e6, 8.0 + (units <= 256 ? 1.15 : 1.6) * n) + 0.1 * units;
         if (p < price) price = p, best = n;
     }
-    return std::max(best, 1);
+    return best;
 }
 
 zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta* st, const StageFixed* fixed,
@@ -518,9 +514,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
         long unit_steps = 0;
         for (const SharedSegment& g : segments)
             unit_steps += (long)((rows_of(g) + upr - 1) / upr) * (((g.end - g.begin + 1) / 2 + slices - 1) / slices);
-        const int unit_tps = slices * shared_unit_steps(unit_steps * ctx->local_kv_heads,
-                                                        ((st->n_attn_items + 7) / 8 * ctx->local_kv_heads + 3) / 4 * 8,
-                                                        (double)tail_pages * ctx->page_bytes, 128 * (ctx->head_dim + 2) * 4.0 / slices);
+        const int unit_tps = slices * shared_unit_steps(unit_steps * ctx->local_kv_heads, (double)tail_pages * ctx->page_bytes);
         for (const SharedSegment& g : segments) {
             std::vector<int> rows;
             for (int s : g.members)

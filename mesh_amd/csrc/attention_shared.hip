@@ -46,14 +46,11 @@ template <int D> struct SharedQ {
             x[ks][1] = *(const f32x4*)(qp + 16 * ks + 4);
         }
     }
-    __device__ __forceinline__ void split(float scale, bf16x8 (&q)[D / 16][3]) const {
+    __device__ __forceinline__ void split(float scale, int ks, bf16x8 (&q)[3]) const {
+        float y[8];
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = x[ks][j >> 2][j & 3] * scale;
-            split3_bf16x8(y, q[ks]);
-        }
+        for (int j = 0; j < 8; ++j) y[j] = x[ks][j >> 2][j & 3] * scale;
+        split3_bf16x8(y, q);
     }
 };
 
@@ -65,7 +62,12 @@ struct SharedPages {
     const int* bt;   // the sequence's table from the unit's first page on
     int last;        // last page of the segment, counted from there
     int base, ids;
-    __device__ __forceinline__ void fetch(int lane) { ids = bt[min(base + lane, last)]; }
+    __device__ __forceinline__ void fetch(int lane) {
+        ids = bt[min(base + lane, last)];
+        // (waited for here, in the rare branch: left pending, the lane reads behind the
+        // branch would wait for every copy in flight, each step)
+        asm volatile("" : "+v"(ids));
+    }
     __device__ __forceinline__ void tile(int rel, int lane, int& pg0, int& pg1) {
         if (2 * rel >= base + 64) {
             base = (2 * rel) & ~63;
@@ -78,18 +80,17 @@ struct SharedPages {
 
 // V rows of keys outside [0, last] enter the product as 0: their weights are 0,
 // but 0 x inf is NaN, and rows before a trimmed window hold whatever they held.
-// Element j of k-step ks2 is key base + 16 ks2 + 8 (j / 4) + 4 h + j % 4.
+// Element j of a fragment is key base + at + 8 (j / 4) + j % 4.
 template <int D>
-__device__ __forceinline__ void shared_mask_v(bf16x8 (&v)[2][D / 32], int base, int h, int last) {
+__device__ __forceinline__ void shared_mask_v(bf16x8 (&v)[D / 32], int base, int at, int last) {
+    asm volatile("" ::: "memory");  // (keeps the caller's branch: the selects cost every tile otherwise)
 #pragma unroll
-    for (int ks2 = 0; ks2 < 2; ++ks2)
+    for (int j = 0; j < 8; ++j) {
+        const int key = base + at + 8 * (j >> 2) + (j & 3);
+        if (key < 0 || key > last)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int key = base + 16 * ks2 + 8 * (j >> 2) + 4 * h + (j & 3);
-            if (key < 0 || key > last)
-#pragma unroll
-                for (int db = 0; db < D / 32; ++db) v[ks2][db][j] = (__bf16)0.0f;
-        }
+            for (int db = 0; db < D / 32; ++db) v[db][j] = (__bf16)0.0f;
+    }
 }
 
 // The key slices' (m, l, O) of each column meet in LDS (slices 1.. write, slice
@@ -158,25 +159,36 @@ __device__ __forceinline__ void shared_finish(const SharedArgs& a, f32x16 (&o)[D
 // bf16 pools.  A workgroup of CW x KW waves owns one kv head of one unit: up to
 // 32 CW columns = (row, q head of the kv head) pairs, 32 per column wave, and a
 // run of 32-key tiles (two pages) of the segment.  Tiles go to the KW key
-// slices in turn; each is copied once into an LDS ring by the CW waves of its
-// slice (buffer loads into LDS, the pool's page order, no registers) and serves
-// all columns.  Per tile and wave, on v_mfma_f32_32x32x16_bf16 (h = lane / 32):
+// slices in turn; each is copied once into LDS by the CW waves of its slice
+// (buffer loads into LDS, the pool's page order, no registers) and serves all
+// columns.  Per tile and wave, on v_mfma_f32_32x32x16_bf16 (h = lane / 32):
 //   S[key][col] = sum_d K[key][d] Q[col][d]; the lane gets key 8 (i / 4) + 4 h + i % 4, i < 16
 //   online softmax per column over the lane's 16 keys and the 16 of lane ^ 32
 //   O[d][col] += sum_key V[key][d] P[key][col]: P's fragment is the lane's own scores
 // Q and P enter in three bf16 parts, which hold all of an f32's 24 bits (two
 // parts, 17 bits, put the result 4e-6 of its norm off: 3.4e-6 from Q, 2.2e-6
 // from P; three leave 1e-7), K and V are exact; sums are f32.
-constexpr size_t unit_lds(int D, int KW, int stages) { return (size_t)stages * KW * 8 * D * 16; }
+//
+// NEXT: step t weighs tile t's scores while the MFMAs form those of tile t + 1
+// (the matrix pipe and the VALU work side by side on one wave's instructions),
+// then adds V^T P of tile t.  K and V have rings of three slots each, K one tile
+// ahead, and at D = 128 the third part of Q lies in LDS: 80 KB, two workgroups a
+// CU, and no spills (a spilled register's reload waits, in order, for the copies
+// issued before it).  Without NEXT two slots and one tile at a time.
+constexpr bool unit_q_in_lds(int D, bool next) { return D == 128 && next; }
+constexpr size_t unit_lds(int D, int CW, int KW, bool next) {
+    return (size_t)(next ? 3 : 2) * KW * 8 * D * 16 + (unit_q_in_lds(D, next) ? (size_t)CW * KW * (D / 16) * 1024 : 0);
+}
 
-template <int D, int CW, int KW, int STAGES>
+template <int D, int CW, int KW, bool NEXT>
 __device__ __forceinline__ void shared_unit(const SharedArgs& a, const int* __restrict__ block_tables, int wg, bf16x8* buf) {
-    constexpr int CHUNKS = 8 * D;        // 16 B chunks per tile: 2 pages x (K, V) x 16 rows x D bf16
-    constexpr int VM = CHUNKS / 64 / CW; // copies (1 KiB each) per wave and tile
+    constexpr int SLOTS = NEXT ? 3 : 2;
+    constexpr int HALF = 4 * D;          // 16 B chunks of a tile's K (or V): 2 pages x 16 rows x D bf16
+    constexpr int VM = HALF / 64 / CW;   // copies (1 KiB each) per wave and half tile
     constexpr int RUN = D / 32;          // 1 KiB runs of one head's K (or V) page
-    static_assert(VM * 64 * CW == CHUNKS, "tile copy split");
-    static_assert(shared_combine_bytes(D, CW, KW) <= unit_lds(D, KW, STAGES), "combine buffer");
-    auto lds = [&](int slot, int slice) { return buf + (size_t)(slot * KW + slice) * CHUNKS; };
+    constexpr bool QLDS = unit_q_in_lds(D, NEXT);
+    static_assert(VM * 64 * CW == HALF, "tile copy split");
+    static_assert(shared_combine_bytes(D, CW, KW) <= (size_t)SLOTS * KW * 2 * HALF * 16, "combine buffer");
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -203,27 +215,41 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const int* __re
     // (keys before the window lie in the segment's first page, before row foff; those past its end in its last tile)
     const int jlast = (pe - pb) * kPageRows - 1;
 
-    const uint16_t* pool = (const uint16_t*)a.pool;
     const int p0 = pb + 2 * kt0;  // the unit's first page
     SharedPages pages{block_tables + (size_t)seq * a.stride + p0, pe - 1 - p0, 0, ids};
-    const size_t kv_tile = (size_t)kPageRows * D;
-    const size_t v_block = (size_t)a.kv_heads * kv_tile;
+    // Copies are buffer loads into LDS over one page: its base in the (scalar)
+    // buffer descriptor, kept from a tile's K for its V, the lane's 16 B and the
+    // wave's run in the vector offset, K or V in the scalar one.
     const uint32_t page_bytes = (uint32_t)(a.page_elems * 2);
-    const int voff = lane * 16;
-    auto issue = [&](int slot, int pg0, int pg1) {
-        const __amdgpu_buffer_rsrc_t r0 =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(pool + (size_t)pg0 * a.page_elems), 0, page_bytes, 0x00020000);
-        const __amdgpu_buffer_rsrc_t r1 =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(pool + (size_t)pg1 * a.page_elems), 0, page_bytes, 0x00020000);
+    const uint32_t k_off = (uint32_t)kvh * (kPageRows * D * 2), v_off = (uint32_t)a.kv_heads * (kPageRows * D * 2) + k_off;
+    auto page_rsrc = [&](int pg) {
+        const unsigned char* at = (const unsigned char*)a.pool + (uint64_t)(uint32_t)pg * page_bytes;
+        return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, page_bytes, 0x00020000);
+    };
+    __amdgpu_buffer_rsrc_t rs0, rs1;  // the two pages of the tile asked for last
+    auto tile = [&](int x) {
+        int pg0, pg1;
+        pages.tile(KW * x + slice, lane, pg0, pg1);
+        rs0 = page_rsrc(pg0);
+        rs1 = page_rsrc(pg1);
+    };
+    auto k_slot = [&](int x) { return buf + (size_t)((x % SLOTS) * KW + slice) * 2 * HALF; };
+    auto v_slot = [&](int x) { return k_slot(x) + HALF; };
+    // the tile's K or V into `to`: the wave takes 1 KiB runs i CW + wq of (page, run)
+    auto issue = [&](bf16x8* to, uint32_t off) {
 #pragma unroll
         for (int i = 0; i < VM; ++i) {
-            const int f = i * CW + wq;  // (page, K or V, 1 KiB run)
-            const int pp = f / (2 * RUN), kv = (f / RUN) & 1, run = f % RUN;
-            const int soff = (int)(((kv ? v_block : 0) + (size_t)kvh * kv_tile) * 2) + run * 1024;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(pp ? r1 : r0, (lds_void*)(lds(slot, slice) + f * 64), 16, voff, soff,
-                                                     0, 0);
+            const int f = i * CW;
+            if constexpr (CW <= RUN) {  // (i, not the wave, tells the page)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(f / RUN ? rs1 : rs0, (lds_void*)(to + (f + wq) * 64), 16,
+                                                         lane * 16 + wq * 1024, off + f % RUN * 1024, 0, 0);
+            } else {  // CW = 2 RUN: a run a wave
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(wq / RUN ? rs1 : rs0, (lds_void*)(to + wq * 64), 16,
+                                                         lane * 16 + wq % RUN * 1024, off, 0, 0);
+            }
         }
     };
+    static_assert(CW <= RUN || CW == 2 * RUN, "a tile's copies by wave");
 
     f32x16 o[D / 32];
 #pragma unroll
@@ -232,76 +258,181 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const int* __re
         for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
     float m = -INFINITY, lsum = 0.0f;
 
-    // step p holds tile kt0 + KW p + slice; the rows' Q goes out behind the first
-    // step's copies
+    // step x holds tile kt0 + KW x + slice; the rows' Q goes out behind the first
+    // tile's copies
     const int nsteps = (kt1 - kt0 + KW - 1) / KW;
+    tile(0);
+    issue(k_slot(0), k_off);
     SharedQ<D> qx;
-    int pg0, pg1;
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        if (s < nsteps) {
-            pages.tile(KW * s + slice, lane, pg0, pg1);
-            issue(s, pg0, pg1);
-        }
-        if (s == 0) qx.load(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h);
+    qx.load(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h);
+    issue(v_slot(0), v_off);
+    if constexpr (NEXT) {  // (V of step x and K of step x + 1 are waited for together)
+        tile(1);
+        issue(k_slot(1), k_off);
+        issue(v_slot(1), v_off);
+        tile(2);
+        issue(k_slot(2), k_off);
     }
-    bf16x8 q[D / 16][3];
-    qx.split(a.scale_log2, q);
+    constexpr int QR = QLDS ? 2 : 3;  // parts of Q in registers
+    bf16x8 q[D / 16][QR];
+    bf16x8* q_lds = buf + (size_t)SLOTS * KW * 2 * HALF + (size_t)wave * (D / 16) * 64 + lane;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        bf16x8 part[3];
+        qx.split(a.scale_log2, ks, part);
+#pragma unroll
+        for (int i = 0; i < QR; ++i) q[ks][i] = part[i];
+        if constexpr (QLDS) q_lds[ks * 64] = part[2];  // (read by this lane alone)
+    }
 
-    for (int t = 0; t < nsteps; ++t) {
-        ring_wait<VM, STAGES - 2>(min(STAGES - 2, nsteps - 1 - t));
-        if (t + STAGES - 1 < nsteps) {
-            pages.tile(KW * (t + STAGES - 1) + slice, lane, pg0, pg1);
-            issue((t + STAGES - 1) % STAGES, pg0, pg1);
+    const int kbase = ((lane >> 4) & 1) * 2 * D + (lane & 15) + h * 16;  // page (l % 32) / 16, row l % 16
+    auto q_part = [&](int ks, int i) -> bf16x8 {
+        if constexpr (QLDS) {
+            if (i == 2) return q_lds[ks * 64];
         }
-        const int kt = kt0 + KW * t + slice;
-        if (busy && kt < kt1) {
-            const bf16x8* st = lds(t % STAGES, slice);
-            const int kbase = ((lane >> 4) & 1) * 2 * (2 * D) + (lane & 15);  // page (l % 32) / 16, row l % 16
-            bf16x8 kf[D / 16];
+        return q[ks][i < QR ? i : 0];
+    };
+    f32x16 s;
+    auto first_scores = [&](int x) {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) kf[ks] = st[kbase + (2 * ks + h) * 16];
-            __builtin_amdgcn_sched_barrier(0);  // the K reads stay ahead of the MFMAs
-            f32x16 s;
+        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+        for (int ks = 0; ks < D / 16; ++ks) {
+            const bf16x8 kf = k_slot(x)[kbase + 2 * ks * 16];
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-#pragma unroll
-                for (int i = 0; i < 3; ++i)
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], q[ks][i], s, 0, 0, 0);
-            }
-            bf16x8 vf[2][D / 32];
-            const bf16x4* sv = (const bf16x4*)st;
-#pragma unroll
-            for (int ks2 = 0; ks2 < 2; ++ks2) {
-                const int vbase = (2 * ks2 + 1) * 4 * D;  // 8-byte units of page ks2's V block
-#pragma unroll
-                for (int db = 0; db < D / 32; ++db) {
-                    const int u = ((db * 4 + h) * 16 + (lane & 15)) * 2 + ((lane >> 4) & 1);
-                    const bf16x4 v0 = sv[vbase + u], v1 = sv[vbase + u + 2 * 16 * 2];
-                    vf[ks2][db] = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);  // the V reads go out before the softmax
-            if (32 * kt < foff || 32 * kt + 31 > jlast) {
-                prefill_mask(s, 32 * kt + 4 * h - foff, jlast - foff);
-                shared_mask_v<D>(vf, 32 * kt - foff, h, jlast - foff);
-            }
-            float pr[16];
-            prefill_softmax<D>(s, o, m, lsum, pr);
-#pragma unroll
-            for (int ks2 = 0; ks2 < 2; ++ks2) {
-                bf16x8 p[3];
-                split3_bf16x8(pr + 8 * ks2, p);
-#pragma unroll
-                for (int i = 0; i < 3; ++i)
-#pragma unroll
-                    for (int db = 0; db < D / 32; ++db)
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], p[i], o[db], 0, 0, 0);
-            }
+            for (int i = 0; i < 3; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q_part(ks, i), s, 0, 0, 0);
         }
+    };
+    if constexpr (NEXT) {
+        ring_barrier<4 * VM>();  // K of step 0: four halves were issued after it
+        if (busy) first_scores(0);
     }
+    for (int t = 0; t < nsteps; ++t) {
+        // V of step t and K of step t + 1 (without NEXT: both of step t) have
+        // arrived, and every wave is done with step t - 1
+        if constexpr (NEXT) {
+            if (t + 1 < nsteps || t == 0) ring_barrier<2 * VM>(); else ring_barrier<0>();
+            if (t + 2 < nsteps) {
+                issue(v_slot(t + 2), v_off);  // its pages are the ones asked for last
+                tile(t + 3);
+                issue(k_slot(t + 3), k_off);
+            }
+        } else {
+            ring_barrier<0>();
+            if (t + 1 < nsteps) {
+                tile(t + 1);
+                issue(k_slot(t + 1), k_off);
+                issue(v_slot(t + 1), v_off);
+            }
+        }
+        if (!busy) continue;
+        const int kt = kt0 + KW * t + slice;
+        const bool edge = 32 * kt < foff || 32 * kt + 31 > jlast || kt >= kt1;
+        const int last = kt < kt1 ? jlast - foff : -1;  // (a slice without a tile in this step sees no key)
+        if constexpr (!NEXT) first_scores(t);
+        if (edge) prefill_mask(s, 32 * kt + 4 * h - foff, last);
+        // The running max follows a tile's only by jumps of more than 8 (log2 units:
+        // P <= 2^8), so O and l are rescaled at the first tile and rarely after.
+        float tmax = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, s[i]);
+        tmax = pair_max(tmax);
+        if (__any(tmax > m + 8.0f)) {
+            const bool up = tmax > m + 8.0f;  // (m = -inf and no visible key: no move, where m - m would be NaN)
+            const float alpha = up ? __builtin_amdgcn_exp2f(m - tmax) : 1.0f;
+            if (up) m = tmax;
+            lsum *= alpha;
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
+        // The tile's 16 weights a lane, in D / 16 pieces, each behind the three MFMAs of
+        // one K fragment of the next tile.  In this order by fences: left to itself
+        // the compiler issues the 24 MFMAs, each waiting for the one before, and
+        // then the VALU work.  (The last step's next tile is what its slot holds,
+        // unused.)
+        f32x16 next;
+        uint32_t pw[2][3][4];           // P's parts, two weights a word
+        constexpr int PIECE = 256 / D;  // weights per piece
+        const bf16x8* k_next = k_slot(t + 1) + kbase;
+        bf16x8 kf;
+        if constexpr (NEXT) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) next[i] = 0.0f;
+            kf = k_next[0];
+        }
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            __builtin_amdgcn_sched_barrier(0);
+            bf16x8 q2, ahead;
+            if constexpr (NEXT) {
+                q2 = q_part(ks, 2);
+                ahead = ks + 1 < D / 16 ? k_next[2 * (ks + 1) * 16] : kf;
+                next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[ks][0], next, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float w[PIECE];
+#pragma unroll
+            for (int e = 0; e < PIECE; ++e) {
+                w[e] = __builtin_amdgcn_exp2f(s[ks * PIECE + e] - mu);
+                lsum += w[e];
+            }
+            if constexpr (NEXT) {
+                __builtin_amdgcn_sched_barrier(0);
+                next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[ks][1], next, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int e = 0; e < PIECE; e += 2) {
+                const int at = ks * PIECE + e;
+                split3_pair(w[e], w[e + 1], pw[at >> 3], (at & 7) >> 1);
+            }
+            if constexpr (NEXT) {
+                __builtin_amdgcn_sched_barrier(0);
+                next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q2, next, 0, 0, 0);
+                kf = ahead;
+            }
+        }
+        bf16x8 p[2][3];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                p[k][i] = __builtin_bit_cast(bf16x8, make_uint4(pw[k][i][0], pw[k][i][1], pw[k][i][2], pw[k][i][3]));
+                // (P is complete here: its work must not sink past the branch below)
+                asm volatile("" ::"v"(p[k][i]));
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        // V^T P by 16 keys: a fragment's registers take the other 16 keys' once its three MFMAs are out
+        const bf16x4* sv = (const bf16x4*)v_slot(t) + (h * 16 + (lane & 15)) * 2 + ((lane >> 4) & 1);
+        auto v_frag = [&](int ks2, int db) {
+            const bf16x4* at = sv + ks2 * 4 * D + db * 128;  // page ks2's V block, in 8-byte units
+            return __builtin_shufflevector(at[0], at[64], 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        bf16x8 vf[D / 32];
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) vf[db] = v_frag(0, db);
+        if (edge) shared_mask_v<D>(vf, 32 * kt - foff, 4 * h, last);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[db], p[0][i], o[db], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            vf[db] = v_frag(1, db);
+        }
+        if (edge) shared_mask_v<D>(vf, 32 * kt - foff, 16 + 4 * h, last);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[db], p[1][i], o[db], 0, 0, 0);
+        if constexpr (NEXT) s = next;
+    }
+    // (copies issued for steps that do not run land before the combine's barrier)
+    ring_barrier<0>();
     shared_finish<D, CW, KW>(a, o, m, lsum, (float*)buf, slice, wq, lane, kvh, item0, nsplits, valid);
 }
 
@@ -391,7 +522,8 @@ __device__ __forceinline__ void shared_unit_f32(const SharedArgs& a, const int* 
     qx.load(a.q + (size_t)grow * a.q_cols + (size_t)(kvh * a.G + g) * D + 8 * h);
     store_split(0);
     bf16x8 q[D / 16][3];
-    qx.split(a.scale_log2, q);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) qx.split(a.scale_log2, ks, q[ks]);
     pages.tile(KW + slice, lane, pg0, pg1);
     load_raw(pg0, pg1);
 
@@ -409,6 +541,10 @@ __device__ __forceinline__ void shared_unit_f32(const SharedArgs& a, const int* 
         }
     };
 
+    auto mask_v = [&](bf16x8 (&v)[2][D / 32], int kt) {
+        shared_mask_v<D>(v[0], 32 * kt - foff, 4 * h, jlast - foff);
+        shared_mask_v<D>(v[1], 32 * kt - foff, 16 + 4 * h, jlast - foff);
+    };
     for (int t = 0; t < nsteps; ++t) {
         ring_barrier<63>();  // the slot is written (LDS only: the next tile's loads stay in flight)
         const int kt = kt0 + KW * t + slice;
@@ -435,7 +571,7 @@ __device__ __forceinline__ void shared_unit_f32(const SharedArgs& a, const int* 
             __builtin_amdgcn_sched_barrier(0);  // the V reads go out before the softmax
             if (edge) {
                 prefill_mask(s, 32 * kt + 4 * h - foff, jlast - foff);
-                shared_mask_v<D>(vf, 32 * kt - foff, h, jlast - foff);
+                mask_v(vf, kt);
             }
             float pr[16];
             prefill_softmax<D>(s, o, m, lsum, pr);
@@ -453,7 +589,7 @@ __device__ __forceinline__ void shared_unit_f32(const SharedArgs& a, const int* 
                             o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks2][db], p[ks2][i], o[db], 0, 0, 0);
                 if (j < 2) {
                     v_frags(st[j + 1], vf);
-                    if (edge) shared_mask_v<D>(vf, 32 * kt - foff, h, jlast - foff);
+                    if (edge) mask_v(vf, kt);
                 }
             }
         }
@@ -575,6 +711,7 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& a, const int* __re
         if (p >= base + 64) {
             base += 64;
             ids = bt[min(base + lane, page_e - 1)];
+            asm volatile("" : "+v"(ids));  // waited for in this branch (SharedPages::fetch)
         }
         load_page(r, __builtin_amdgcn_readlane(ids, p - base));
     };
@@ -670,13 +807,13 @@ __device__ __forceinline__ bool shared_split(const SharedArgs& a, int& unit_wg, 
     return tail_group < 0;
 }
 
-template <int D, int CW, int KW, int STAGES, int RING>
+template <int D, int CW, int KW, bool NEXT, int RING>
 __global__ __launch_bounds__(256, 2) void shared_attention_kernel(SharedArgs a, const int* __restrict__ block_tables) {
-    constexpr size_t bytes = unit_lds(D, KW, STAGES) > tail_lds(D) ? unit_lds(D, KW, STAGES) : tail_lds(D);
+    constexpr size_t unit = unit_lds(D, CW, KW, NEXT), bytes = unit > tail_lds(D) ? unit : tail_lds(D);
     __shared__ bf16x8 buf[bytes / 16];
     int unit_wg, tail_group;
     if (shared_split(a, unit_wg, tail_group))
-        shared_unit<D, CW, KW, STAGES>(a, block_tables, unit_wg, buf);
+        shared_unit<D, CW, KW, NEXT>(a, block_tables, unit_wg, buf);
     else
         shared_tail<uint16_t, D, RING>(a, block_tables, tail_group, buf);
 }
@@ -796,11 +933,11 @@ static void launch_shared(zr_context* ctx, StagedMeta* st, const SharedArgs& a, 
     if (ctx->desc.kv_dtype == ZR_DTYPE_F32)
         hipLaunchKernelGGL((shared_attention_f32_kernel<D, 4>), grid, block, 0, ctx->stream, a, st->block_tables);
     else if (st->unit_cols == 128)
-        hipLaunchKernelGGL((shared_attention_kernel<D, 4, 1, 3, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
+        hipLaunchKernelGGL((shared_attention_kernel<D, 4, 1, true, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
     else if (st->unit_cols == 64)
-        hipLaunchKernelGGL((shared_attention_kernel<D, 2, 2, D == 64 ? 3 : 2, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
+        hipLaunchKernelGGL((shared_attention_kernel<D, 2, 2, D == 64, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
     else
-        hipLaunchKernelGGL((shared_attention_kernel<D, 1, 4, 2, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
+        hipLaunchKernelGGL((shared_attention_kernel<D, 1, 4, false, RING>), grid, block, 0, ctx->stream, a, st->block_tables);
 }
 
 zr_status launch_shared_attention(zr_context* ctx, StagedMeta* st, int layer, const float* q) {

@@ -88,6 +88,19 @@ __device__ inline void split3_bf16x8(const float* x, bf16x8 (&p)[3]) {
     }
 }
 
+// ... of two values, as word `at` of the parts
+__device__ inline void split3_pair(float a, float b, uint32_t (&p)[3][4], int at) {
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
+    typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+    f32x2 v = {a, b};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const bf16x2 h = __builtin_convertvector(v, bf16x2);
+        if (k < 2) v -= __builtin_convertvector(h, f32x2);
+        p[k][at] = __builtin_bit_cast(uint32_t, h);
+    }
+}
+
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 
 __device__ inline float pair_max(float x) {

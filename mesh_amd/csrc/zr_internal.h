@@ -373,7 +373,6 @@ struct StagedMeta {
 // rows | splits << 16, first page of the segment}, {first key tile, end key tile, partial item, end page}, the unit's
 // first 64 pages (the last one repeated), its query rows (likewise), up to 128.
 constexpr int kUnitPages = 8, kUnitRows = 72, kUnitInts = 200;
-constexpr int kSharedSlots = 512;  // resident workgroups of that launch: two per CU
 
 // A run of pages that the block tables of `members` all name at [begin, end).
 struct SharedSegment {
