@@ -393,6 +393,35 @@ zr_status zr_sample(zr_context* ctx, const float* d_logits, int rows, int cols, 
  * and the batched decode path. */
 zr_status zr_sample_last_logits(zr_context* ctx, int rows, const float* temperature, const float* top_p,
                                 const uint64_t* seeds, uint32_t* out_tokens);
+/* Drafted tokens against the target's logits (speculative sampling).  Sequence s
+ * has draft_len[s] = k drafts (0..255) and k + 1 rows of d_logits
+ * [sum (k + 1), cols] f32: row i is the target's at the place of draft i, the last
+ * the one after them.  With p_i = softmax(x_i / temperature) (temperature <= 0:
+ * certain of the argmax), q_i the draft's probabilities and u_i the row's uniform
+ * in [0, 1): draft i is accepted while u_i q_i(y_i) < p_i(y_i); at the first
+ * rejected one a token is drawn from max(p_i - q_i, 0) normalised, after k accepted
+ * ones from p_k: the first index whose cumulative weight exceeds the last row's
+ * u times the whole.  d_draft_probs NULL: the drafts were certain (q_i(y_i) = 1;
+ * looked up, or greedy).  d_out_tokens [num_seqs][out_stride] (out_stride > every
+ * k): the accepted drafts, the drawn token, then 0xffffffff; d_accepted
+ * [num_seqs]: the number accepted.  A logit that is not a number counts as -inf, a
+ * draft outside the columns and a probability below 0 as probability 0; a row
+ * without a finite logit gives token 0.  Weights and sums in f64, in a fixed
+ * order.  cols <= 2^24.  The arrays marked host are read before the call
+ * returns; zr_verify_async enqueues the rest on the context stream.  No
+ * counterpart in the reference (one token a step). */
+typedef struct {
+    int num_seqs;
+    const int* draft_len;        /* host [num_seqs] */
+    const uint32_t* d_drafts;    /* device [sum draft_len] (nullable where that is 0) */
+    const float* d_draft_probs;  /* device [sum draft_len, cols] or NULL */
+    const float* temperature;    /* host [num_seqs] */
+    const float* d_uniforms;     /* device [sum (draft_len + 1)] */
+} zr_verify_batch;
+zr_status zr_verify(zr_context* ctx, const float* d_logits, int cols, const zr_verify_batch* vb,
+                    uint32_t* d_out_tokens, int out_stride, int* d_accepted);
+zr_status zr_verify_async(zr_context* ctx, const float* d_logits, int cols, const zr_verify_batch* vb,
+                          uint32_t* d_out_tokens, int out_stride, int* d_accepted);
 /* y = rms_norm(x) * gamma (tensor_ops.rs:285-304), device f32 [rows, cols]. */
 zr_status zr_rms_norm(zr_context* ctx, const float* d_x, const float* d_gamma, float* d_y, int rows,
                       int cols);

@@ -8,10 +8,10 @@ from .provider import (BackendMicrobatchExecutor, DecodeMicrobatchOutput, Decode
                        DecodePipeline, DeviceBuffer, DeviceContext, ExecutionProviderKind, FastPathPlanner, KVCacheBlob,
                        KVCacheSnapshot, KVCacheWireSnapshot, KVSequenceState, KVTransfer, ModelGeometry,
                        RocmExecutionBackend,
-                       bf16_bits, device_info, executor_contract, probe_provider)
+                       bf16_bits, device_info, executor_contract, probe_provider, verify_device)
 
 __all__ = ["BackendMicrobatchExecutor", "DecodeMicrobatchOutput", "DecodeMicrobatchRequest", "DecodePipeline",
            "DeviceBuffer",
            "DeviceContext", "ExecutionProviderKind", "FastPathPlanner", "KVCacheBlob", "KVCacheSnapshot",
            "KVCacheWireSnapshot", "KVSequenceState", "KVTransfer", "ModelGeometry", "RocmExecutionBackend", "bf16_bits",
-           "device_info", "executor_contract", "probe_provider"]
+           "device_info", "executor_contract", "probe_provider", "verify_device"]

@@ -73,6 +73,11 @@ class PrefixInfo(C.Structure):
                 ("pages_saved", C.c_int)]
 
 
+class VerifyBatch(C.Structure):
+    _fields_ = [("num_seqs", C.c_int), ("draft_len", c_int_p), ("d_drafts", C.c_void_p), ("d_draft_probs", C.c_void_p),
+                ("temperature", c_f32_p), ("d_uniforms", C.c_void_p)]
+
+
 class ExecutorContract(C.Structure):
     _fields_ = [("executor_class", C.c_char_p), ("optimization_profile", C.c_char_p),
                 ("n_host_kernels", C.c_int), ("host_kernels", C.POINTER(C.c_char_p)),
@@ -164,6 +169,9 @@ SIGNATURES = [
     ("zr_sample", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, c_f32_p, c_f32_p, C.POINTER(C.c_uint64),
                             C.c_void_p]),
     ("zr_sample_last_logits", C.c_int, [C.c_void_p, C.c_int, c_f32_p, c_f32_p, C.POINTER(C.c_uint64), c_u32_p]),
+    ("zr_verify", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(VerifyBatch), C.c_void_p, C.c_int, C.c_void_p]),
+    ("zr_verify_async", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(VerifyBatch), C.c_void_p, C.c_int,
+                                  C.c_void_p]),
     ("zr_rms_norm", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
     ("zr_gemm", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]),
     ("zr_gemm_swiglu", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]),

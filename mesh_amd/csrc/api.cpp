@@ -1037,6 +1037,7 @@ void zr_context_destroy(zr_context* ctx) {
     if (ctx->cbor_ws) (void)hipFree(ctx->cbor_ws);
     if (ctx->cbor_out) (void)hipFree(ctx->cbor_out);
     if (ctx->sample_ws_own) (void)hipHostFree(ctx->sample_ws_own);
+    if (ctx->verify_ws) (void)hipFree(ctx->verify_ws);
     free_ctx_buffers(ctx);
     destroy_streams(ctx);
     delete ctx;
@@ -2146,6 +2147,42 @@ zr_status zr_sample_last_logits(zr_context* ctx, int rows, const float* temperat
     ZR_HIP(ctx, hipMemcpyAsync(out_tokens, ctx->tokens_out, 4 * (size_t)rows, hipMemcpyDeviceToHost, ctx->stream));
     ZR_HIP(ctx, hipStreamSynchronize(ctx->stream));
     return ZR_OK;
+}
+
+static zr_status verify_check(zr_context* ctx, const void* d_logits, int cols, const zr_verify_batch* vb, const void* d_out,
+                              int out_stride, const void* d_accepted) {
+    if (!d_logits || !vb || !d_out || !d_accepted || !vb->draft_len || !vb->temperature || !vb->d_uniforms)
+        return set_err(ctx, ZR_E_INVALID, "null argument");
+    if (vb->num_seqs <= 0) return set_err(ctx, ZR_E_INVALID, "verification of %d sequences", vb->num_seqs);
+    if (cols <= 0 || cols > (1 << 24)) return set_err(ctx, ZR_E_INVALID, "%d columns outside 1..2^24", cols);
+    long rows = 0;
+    int most = 0;
+    for (int s = 0; s < vb->num_seqs; ++s) {
+        const int k = vb->draft_len[s];
+        if (k < 0 || k > 255) return set_err(ctx, ZR_E_INVALID, "sequence %d has %d drafts (0..255)", s, k);
+        if (vb->temperature[s] != vb->temperature[s])
+            return set_err(ctx, ZR_E_INVALID, "sequence %d has a temperature that is not a number", s);
+        most = std::max(most, k);
+        rows += k + 1;
+    }
+    if (rows > vb->num_seqs && !vb->d_drafts) return set_err(ctx, ZR_E_INVALID, "null argument");
+    if (out_stride <= most) return set_err(ctx, ZR_E_INVALID, "output stride %d for %d drafts and a token", out_stride, most);
+    return ZR_OK;
+}
+
+zr_status zr_verify_async(zr_context* ctx, const float* d_logits, int cols, const zr_verify_batch* vb,
+                          uint32_t* d_out_tokens, int out_stride, int* d_accepted) {
+    if (!ctx) return set_global_err(ZR_E_INVALID, "null argument");
+    if (zr_status rc = verify_check(ctx, d_logits, cols, vb, d_out_tokens, out_stride, d_accepted)) return rc;
+    ZR_HIP(ctx, hipSetDevice(ctx->device));
+    return launch_verify(ctx, d_logits, cols, vb, d_out_tokens, out_stride, d_accepted);
+}
+
+zr_status zr_verify(zr_context* ctx, const float* d_logits, int cols, const zr_verify_batch* vb, uint32_t* d_out_tokens,
+                    int out_stride, int* d_accepted) {
+    zr_status rc = zr_verify_async(ctx, d_logits, cols, vb, d_out_tokens, out_stride, d_accepted);
+    if (!rc) ZR_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    return rc;
 }
 
 zr_status zr_rms_norm(zr_context* ctx, const float* d_x, const float* d_gamma, float* d_y, int rows, int cols) {

@@ -254,6 +254,8 @@ struct zr_context {
     size_t cbor_out_bytes = 0;
     void* sample_ws = nullptr;      // stochastic sampling: per-row parameters (pinned host memory)
     size_t sample_ws_bytes = 0;
+    void* verify_ws = nullptr;      // draft verification: chunk statistics, sums of the rest
+    size_t verify_ws_bytes = 0;
     void* sample_ws_own = nullptr;  // ... of calls with more rows than the context's own block holds
     // Device-fed token ids out of the vocabulary: the embedding kernel keeps
     // the smallest (row << 32 | id) here (all ones = none); a forward pass fed
@@ -473,6 +475,10 @@ constexpr size_t kSampleArgBytes = 32;  // per-row parameters of launch_sample
 // sample_tokens_device_with_seeds per row (sample.hip); parameters are host arrays
 zr_status launch_sample(zr_context* ctx, const float* d_logits, int rows, int cols, const float* temperature,
                         const float* top_p, const uint64_t* seeds, uint32_t* d_out);
+
+// zr_verify_async (checked arguments)
+zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const zr_verify_batch* vb, uint32_t* d_out,
+                        int out_stride, int* d_accepted);
 
 enum GemmEpilogue { kEpiStore = 0, kEpiSwiGLU = 1 };
 struct GemmPlan {

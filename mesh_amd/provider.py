@@ -49,7 +49,8 @@ FUSED_KERNEL_STAGES = {
                         "shared_attention_kernel", "shared_attention_f32_kernel", "shared_merge_kernel"],
     "residual_mlp": ["rms_norm_vec_kernel", "rms_norm_kernel", "gemm_kernel", "gemm_swiglu_ksplit_kernel",
                      "splitk_reduce_kernel"],
-    "device_sampling": ["argmax_partial_kernel", "argmax_final_kernel", "sample_kernel"],
+    "device_sampling": ["argmax_partial_kernel", "argmax_final_kernel", "sample_kernel", "verify_stats_kernel",
+                        "verify_residual_kernel", "verify_emit_kernel"],
 }
 
 
@@ -735,6 +736,47 @@ def sample_device(ctx: "DeviceContext", logits: np.ndarray, temperature, top_p, 
         d_x.free()
         d_out.free()
     return [int(t) for t in out]
+
+
+def verify_device(ctx: "DeviceContext", logits: np.ndarray, drafts: Sequence[Sequence[int]], temperature,
+                  uniforms: np.ndarray, draft_probs: Optional[np.ndarray] = None):
+    """Drafted tokens against the target's logits on the GPU (zr_verify): logits
+    [sum (k + 1), cols] with k = len(drafts[s]), uniforms one per row, draft_probs
+    [sum k, cols] or None (certain drafts).  Returns (tokens, accepted): per
+    sequence its accepted drafts and the token drawn after them, and how many
+    were accepted."""
+    x = np.ascontiguousarray(logits, np.float32)
+    lens = np.ascontiguousarray([len(d) for d in drafts], np.int32)
+    flat = np.ascontiguousarray([t for d in drafts for t in d], np.uint32)
+    temps = np.ascontiguousarray(temperature, np.float32)
+    u = np.ascontiguousarray(uniforms, np.float32)
+    n, rows = lens.size, int(lens.sum()) + lens.size
+    if x.ndim != 2 or x.shape[0] != rows or u.size != rows or temps.size != n:
+        raise ZrError(-1, f"verification of {n} sequences with {rows} rows: logits {x.shape}, {u.size} uniforms, "
+                          f"{temps.size} temperatures")
+    stride = int(lens.max()) + 1 if n else 1
+    bufs = [DeviceBuffer.from_numpy(ctx, x), DeviceBuffer.from_numpy(ctx, u)]
+    d_y = d_q = None
+    if flat.size:
+        d_y = DeviceBuffer.from_numpy(ctx, flat)
+        bufs.append(d_y)
+    if draft_probs is not None and flat.size:
+        q = np.ascontiguousarray(draft_probs, np.float32)
+        if q.shape != (flat.size, x.shape[1]):
+            raise ZrError(-1, f"draft probabilities {q.shape} for {flat.size} drafts of {x.shape[1]} columns")
+        d_q = DeviceBuffer.from_numpy(ctx, q)
+        bufs.append(d_q)
+    out, acc = DeviceBuffer(ctx, 4 * max(n, 1) * stride), DeviceBuffer(ctx, 4 * max(n, 1))
+    bufs += [out, acc]
+    try:
+        vb = _lib.VerifyBatch(n, _ptr(lens, C.c_int), d_y.ptr if d_y else None, d_q.ptr if d_q else None,
+                              _ptr(temps, C.c_float), bufs[1].ptr)
+        ctx.check(ctx.lib.zr_verify(ctx.h, bufs[0].ptr, x.shape[1], C.byref(vb), out.ptr, stride, acc.ptr))
+        tokens, accepted = out.download(np.uint32, (n, stride)), acc.download(np.int32, (n,))
+    finally:
+        for b in bufs:
+            b.free()
+    return [tokens[s, :accepted[s] + 1].tolist() for s in range(n)], accepted.tolist()
 
 
 @dataclass
