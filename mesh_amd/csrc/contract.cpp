@@ -19,7 +19,7 @@ const char* const kStageKernels[] = {
     "paged_attention_kernel,paged_prefill_attention_kernel,attention_merge_kernel,shared_attention_kernel,"
     "shared_attention_f32_kernel,shared_merge_kernel",
     "rms_norm_vec_kernel,rms_norm_kernel,gemm_kernel,gemm_swiglu_ksplit_kernel,splitk_reduce_kernel",
-    "argmax_partial_kernel,argmax_final_kernel,sample_kernel,verify_stats_kernel,verify_residual_kernel,"
+    "argmax_partial_kernel,argmax_final_kernel,sample_kernel,verify_stats_kernel,verify_rest_kernel,"
     "verify_emit_kernel",
 };
 const char* const kHostKernels[] = {"host_assisted_sampling"};

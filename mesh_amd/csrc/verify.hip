@@ -14,17 +14,23 @@
 // Then every emitted token has the target's distribution.
 //
 // A token changes where two cumulative sums of a vocabulary's weights change
-// places, so weights and sums are held in f64 (a sum off by 1e-8 would change one
-// token in a thousand of a vocabulary of 128256; these are off by about 1e-13).
+// places: the emission row's weights and sums are held in f64 (a sum off by 1e-8
+// would change one token in a thousand of a vocabulary of 128256; these are off by
+// about 1e-13).  A draft's test has one border alone, so the other rows' sums Z are
+// f32 weights' (1e-7 of Z): of k + 1 rows one is weighed in f64, whose exp costs
+// about 20 f64 operations a logit, more than the logit's bytes (stats in f64: 56 us
+// of 64 x 5 rows x 128256, in f32 at the rate of the bytes).
 //
-//   verify_stats_kernel     one pass over all logits: per chunk of a row its largest
-//                           logit, the first place of it, and the sum of weights
-//                           relative to it.  HBM bound: 4 bytes a logit against
-//                           about 20 f64 operations, which take three quarters of
-//                           the bytes' time at full rate.
-//   verify_residual_kernel  per chunk of the rejected row: sum max(w - q Z, 0)
-//   verify_emit_kernel      the crossing's chunk by the chunks' sums, then its
-//                           place in the chunk, which is read again
+//   verify_stats_kernel  one pass over all logits: per chunk of a row its largest
+//                        logit, the first place of it, and the f32 sum of weights
+//                        relative to it.  HBM bound.
+//   verify_rest_kernel   the tests, then per chunk of the emission row in f64:
+//                        W = sum w, and over A = {w > q Z} the sums of w and q.
+//                        The rest's weight is then W_A - Q_A Z with the f64 Z =
+//                        sum W: a column that the f32 Z puts on the wrong side of A
+//                        weighs below 1e-7 of itself.
+//   verify_emit_kernel   the crossing's chunk by the chunks' sums, then its place in
+//                        the chunk, which is weighed again
 #include "zr_internal.h"
 
 namespace zr {
@@ -33,7 +39,9 @@ namespace {
 
 constexpr int kSeqs = 256;        // sequences a launch (their lengths and temperatures are kernel arguments)
 constexpr int kMaxDrafts = 255;   // drafts of one sequence
+constexpr int kRestChunk = 2048;  // columns of an emission row's chunk
 constexpr double kNothing = -1000.0;  // exp of it is 0
+constexpr float kLog2E = 1.44269504088896341f;
 
 struct VerifyArgs {
     int row[kSeqs + 1];    // first logits row of each sequence, and the end; drafts before it: row[s] - s
@@ -47,23 +55,43 @@ struct VerifyBufs {
     const float* probs;    // [drafts, cols] or null
     const float* u;        // [rows]
     struct ChunkStat* stat;  // [rows][chunks]
-    double* resid;         // [n][chunks]
+    struct RestSum* rest;    // [n][rest_chunks]
+    struct Decision* dec;    // [n]
+    int rest_chunks;
     uint32_t* out;
     int out_stride;
     int* accepted;
 };
 
 struct ChunkStat {
-    float m;     // largest logit of the chunk (-inf: none)
-    int at;      // its first column
-    double sum;  // of exp((x - m) / T)
+    float m;    // largest logit of the chunk (-inf: none)
+    int at;     // its first column
+    float sum;  // of exp((x - m) / T)
+    int pad;
 };
 
-// exp(y) for y <= 0 by y = k ln 2 + r, |r| <= ln 2 / 2, and the Taylor series of
-// exp(r) to r^10 (the next term is below 2.2e-13)
+struct RestSum {
+    double w, wa, qa;  // sum of w; over the columns with w > q Z: of w and of q
+};
+
+// What the tests of a sequence come to.
+struct Decision {
+    int drafts, accepted, row;  // drafts of the sequence; accepted ones; the row the token comes from
+    float m;                    // ... its largest logit
+    int at;                     // ... the first place of it
+    float z;                    // ... the f32 sum of its weights (0: none weighs)
+    float t;
+    int pad;
+};
+
+// exp(y) for y <= 0: y = k ln 2 + r, |r| <= ln 2 / 2 (k by adding and taking away
+// 1.5 2^52, which leaves it in the sum's low bits; ln 2 in two parts, Cody and
+// Waite's, k times the first exact), and the Taylor series of exp(r) to r^10 (the
+// next term is below 2.2e-13).  0 below -700.
 __device__ inline double exp_neg(double y) {
-    const double k = __builtin_rint(y * 1.4426950408889634074);
-    double r = __builtin_fma(-k, 0.693147180369123816490, y);  // ln 2 in two parts: k times the first is exact
+    constexpr double kRound = 6755399441055744.0;
+    const double t = __builtin_fma(y, 1.4426950408889634074, kRound), k = t - kRound;
+    double r = __builtin_fma(-k, 0.693147180369123816490, y);
     r = __builtin_fma(-k, 1.90821492927058770002e-10, r);
     double e = 1.0 / 3628800;
     e = __builtin_fma(e, r, 1.0 / 362880);
@@ -76,7 +104,8 @@ __device__ inline double exp_neg(double y) {
     e = __builtin_fma(e, r, 0.5);
     e = __builtin_fma(e, r, 1.0);
     e = __builtin_fma(e, r, 1.0);
-    return __builtin_ldexp(e, (int)k);
+    const double scaled = __hiloint2double(__double2hiint(e) + (__double2loint(t) << 20), __double2loint(e));  // e 2^k
+    return y >= -700.0 ? scaled : 0.0;
 }
 
 // weight of a logit against the largest one, m: exp((x - m) / T); 0 for -inf and
@@ -85,17 +114,17 @@ __device__ inline double weight(float x, float m, double inv_t) {
     const double y = __builtin_fmax(((double)x - (double)m) * inv_t, kNothing);  // (NaN: kNothing)
     return x == m ? 1.0 : exp_neg(y);
 }
+// the same in f32: c = log2(e) / T
+__device__ inline float weight32(float x, float m, float c) {
+    const float y = fmaxf((x - m) * c, -1000.0f);  // (NaN: nothing)
+    return x == m ? 1.0f : __builtin_amdgcn_exp2f(y);
+}
 
 __device__ inline double shfl_xor64(double v, int mask) {
     return __hiloint2double(__shfl_xor(__double2hiint(v), mask, 64), __shfl_xor(__double2loint(v), mask, 64));
 }
 __device__ inline double shfl_up64(double v, int by) {
     return __hiloint2double(__shfl_up(__double2hiint(v), by, 64), __shfl_up(__double2loint(v), by, 64));
-}
-__device__ inline double wave_sum(double v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += shfl_xor64(v, off);
-    return v;
 }
 // the larger logit, the lower column among equals
 __device__ inline void take_larger(float& m, int& at, float m2, int at2) {
@@ -124,7 +153,7 @@ template <int E, bool VEC>
 __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyArgs v, int n) {
     __shared__ float sm[4];
     __shared__ int sat[4];
-    __shared__ double ss[4];
+    __shared__ float ss[4];
     const int row = blockIdx.x / b.chunks, ch = blockIdx.x - row * b.chunks;
     const float t = v.temp[seq_of(v, n, row)];
     const int c0 = ch * b.chunk, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -159,18 +188,20 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyA
         }
     }
     wave_larger(m, at);
-    double sum = 0.0;
+    float sum = 0.0f;
+    const float c = kLog2E / t;
     if (t > 0.0f && m != -INFINITY) {
-        const double inv_t = 1.0 / (double)t;
-        double s2 = 0.0;
+        float s2 = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            sum += weight(d[e].x, m, inv_t);
-            s2 += weight(d[e].y, m, inv_t);
-            sum += weight(d[e].z, m, inv_t);
-            s2 += weight(d[e].w, m, inv_t);
+            sum += weight32(d[e].x, m, c);
+            s2 += weight32(d[e].y, m, c);
+            sum += weight32(d[e].z, m, c);
+            s2 += weight32(d[e].w, m, c);
         }
-        sum = wave_sum(sum + s2);
+        sum += s2;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
     }
     if (lane == 0) {
         sm[wave] = m;
@@ -181,200 +212,227 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyA
     if (tid) return;
 #pragma unroll
     for (int w = 1; w < 4; ++w) take_larger(m, at, sm[w], sat[w]);
-    double all = 0.0;
+    float all = 0.0f;
     if (t > 0.0f && m != -INFINITY)
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-            if (sm[w] != -INFINITY) all += ss[w] * weight(sm[w], m, 1.0 / (double)t);
-    b.stat[(size_t)row * b.chunks + ch] = {m, at, all};
+            if (sm[w] != -INFINITY) all += ss[w] * weight32(sm[w], m, c);
+    b.stat[(size_t)row * b.chunks + ch] = {m, at, all, 0};
 }
 
-// What a workgroup of the later kernels finds out about its sequence first.
-struct Decision {
-    int drafts, accepted, row;  // drafts of the sequence; accepted ones; the row the token comes from
-    float m;                    // ... its largest logit
-    int at;                     // ... the first place of it
-    double z;                   // ... and its weights' sum
-    float t;
-};
-
-// Each wave takes rows of the sequence in turn: their chunks' sums joined (in
-// one order, so every workgroup gets the same bits), then the row's test.
-template <int WAVES>
+// The tests of a sequence, by 16 groups of 16 lanes, a row each in turn: the
+// chunks' sums joined in one order, so every workgroup gets the same bits.  The
+// draft's own logit and probability come beside them.
 __device__ inline Decision decide(const VerifyBufs& b, const VerifyArgs& v, int s) {
-    __shared__ float sm[kMaxDrafts + 1];
-    __shared__ int sat[kMaxDrafts + 1];
-    __shared__ double sz[kMaxDrafts + 1];
-    __shared__ int ok[kMaxDrafts + 1];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ float sm[kMaxDrafts + 1], sz[kMaxDrafts + 1];
+    __shared__ int sat[kMaxDrafts + 1], ok[kMaxDrafts + 1];
+    const int tid = threadIdx.x, lane = tid & 15;
     const int row0 = v.row[s], k = v.row[s + 1] - row0 - 1, d0 = row0 - s;
-    const float t = v.temp[s];
-    const double inv_t = 1.0 / (double)t;
-    for (int i = wave; i <= k; i += WAVES) {
+    const float t = v.temp[s], c32 = kLog2E / t;
+    for (int i = tid >> 4; i <= k; i += 16) {
+        const uint32_t y = i < k ? b.drafts[d0 + i] : 0xffffffffu;
+        const bool in = y < (uint32_t)b.cols;  // (an id outside the vocabulary has no probability)
+        const float xy = in ? b.logits[(size_t)(row0 + i) * b.cols + y] : -INFINITY;
+        const float qy = !in ? 0.0f : b.probs ? fmaxf(b.probs[(size_t)(d0 + i) * b.cols + y], 0.0f) : 1.0f;
+        const float u = b.u[row0 + i];
         const ChunkStat* st = b.stat + (size_t)(row0 + i) * b.chunks;
         float m = -INFINITY;
-        int at = 0;
-        for (int c = lane; c < b.chunks; c += 64) {
+        int at = 0x7fffffff;
+        for (int c = lane; c < b.chunks; c += 16) {
             const ChunkStat x = st[c];
             if (x.m > m) {
                 m = x.m;
                 at = x.at;
             }
         }
-        if (m == -INFINITY) at = 0x7fffffff;
-        wave_larger(m, at);
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) take_larger(m, at, __shfl_xor(m, off, 64), __shfl_xor(at, off, 64));
         if (m == -INFINITY) at = 0;  // a row without a finite logit: the first place, as the argmax has it
-        double z = 0.0;
-        if (t > 0.0f && m != -INFINITY) {
-            for (int c = lane; c < b.chunks; c += 64) {
+        float z = 0.0f;
+        if (t > 0.0f && m != -INFINITY)
+            for (int c = lane; c < b.chunks; c += 16) {
                 const ChunkStat x = st[c];
-                if (x.m != -INFINITY) z += x.sum * weight(x.m, m, inv_t);
+                if (x.m != -INFINITY) z += x.sum * weight32(x.m, m, c32);
             }
-            z = wave_sum(z);
-        }
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) z += __shfl_xor(z, off, 64);
         if (lane == 0) {
-            bool yes = false;
-            if (i < k) {
-                const uint32_t y = b.drafts[d0 + i];
-                if (t <= 0.0f) {
-                    yes = y == (uint32_t)at;
-                } else if (y < (uint32_t)b.cols) {  // (an id outside the vocabulary has no probability)
-                    const double q = b.probs ? (double)fmaxf(b.probs[(size_t)(d0 + i) * b.cols + y], 0.0f) : 1.0;
-                    const double w = m == -INFINITY ? 0.0 : weight(b.logits[(size_t)(row0 + i) * b.cols + y], m, inv_t);
-                    yes = (double)b.u[row0 + i] * q * z < w;
-                }
-            }
             sm[i] = m;
             sat[i] = at;
             sz[i] = z;
-            ok[i] = yes;
+            ok[i] = t <= 0.0f ? y == (uint32_t)at
+                              : m != -INFINITY && (double)u * (double)qy * (double)z < weight(xy, m, 1.0 / (double)t);
         }
     }
     __syncthreads();
     int a = 0;
     while (a < k && ok[a]) ++a;
-    return {k, a, row0 + a, sm[a], sat[a], sz[a], t};
+    return {k, a, row0 + a, sm[a], sat[a], sz[a], t, 0};
 }
 
-// The weight a token of the emission row is drawn with: of p, or of the rest that
-// the rejected draft leaves.
+// Where the emission row's weights come from: of p, or of the rest that the
+// rejected draft leaves.
 struct Rest {
     const float* x;
-    const float* q;     // the rejected draft's probabilities; null: p, without column `out`
-    uint32_t out;       // a certain draft's own column (none: 0xffffffff)
-    float m;
-    double z, inv_t;
-    __device__ inline double operator()(int c) const {
-        const double w = weight(x[c], m, inv_t);
-        if (q) return __builtin_fmax(w - (double)fmaxf(q[c], 0.0f) * z, 0.0);
-        return (uint32_t)c == out ? 0.0 : w;
-    }
+    const float* q;  // the rejected draft's probabilities, or null: p ...
+    uint32_t out;    // ... without a certain draft's own column (none: 0xffffffff)
 };
-
 __device__ inline Rest rest_of(const VerifyBufs& b, const VerifyArgs& v, int s, const Decision& d) {
     const size_t at = (size_t)(v.row[s] - s + d.accepted);
     const bool left = d.accepted < d.drafts;
     return {b.logits + (size_t)d.row * b.cols, left && b.probs ? b.probs + at * b.cols : nullptr,
-            left && !b.probs ? b.drafts[at] : 0xffffffffu, d.m, d.z, 1.0 / (double)d.t};
+            left && !b.probs ? b.drafts[at] : 0xffffffffu};
 }
 
-// Sums of the rest over the chunks of every sequence whose token needs them (a
-// rejected draft with probabilities).
-__global__ __launch_bounds__(256) void verify_residual_kernel(VerifyBufs b, VerifyArgs v) {
-    __shared__ double ss[4];
-    const int s = blockIdx.x / b.chunks, ch = blockIdx.x - s * b.chunks;
-    if (v.temp[s] <= 0.0f) return;
-    const Decision d = decide<4>(b, v, s);
-    if (d.accepted == d.drafts || d.z <= 0.0) return;
-    const Rest rest = rest_of(b, v, s, d);
-    const int c1 = min((ch + 1) * b.chunk, b.cols);
-    double sum = 0.0;
-#pragma unroll 4
-    for (int c = ch * b.chunk + threadIdx.x; c < c1; c += 256) sum += rest(c);
-    sum = wave_sum(sum);
-    if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = sum;
+__device__ inline double wave_sum(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += shfl_xor64(v, off);
+    return v;
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyArgs v) {
+    __shared__ double ss[3][4];
+    constexpr int E = kRestChunk / 256;
+    const int s = blockIdx.x / b.rest_chunks, ch = blockIdx.x - s * b.rest_chunks, tid = threadIdx.x;
+    const Decision d = decide(b, v, s);
+    if (ch == 0 && tid == 0) b.dec[s] = d;
+    if (d.t <= 0.0f || d.z <= 0.0f) return;  // greedy, or nothing weighs: the first largest logit
+    const Rest r = rest_of(b, v, s, d);
+    const int c0 = ch * kRestChunk;
+    float x[E], q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        x[e] = -INFINITY;
+        q[e] = 0.0f;
+    }
+    if constexpr (VEC) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const int c = c0 + e * 256 + tid * 4;
+            if (c < b.cols) {
+                *(float4*)(x + e) = *(const float4*)(r.x + c);
+                if (r.q) *(float4*)(q + e) = *(const float4*)(r.q + c);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int c = c0 + e * 256 + tid;
+            if (c < b.cols) {
+                x[e] = r.x[c];
+                if (r.q) q[e] = r.q[c];
+            }
+        }
+    }
+    const double inv_t = 1.0 / (double)d.t, z = d.z;
+    double w = 0.0, wa = 0.0, qa = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int c = VEC ? c0 + (e / 4) * 1024 + tid * 4 + (e & 3) : c0 + e * 256 + tid;
+        const double we = weight(x[e], d.m, inv_t), qe = fmaxf(q[e], 0.0f);
+        w += we;
+        const bool in = r.q ? we > qe * z : (uint32_t)c != r.out;
+        wa += in ? we : 0.0;
+        qa += in ? qe : 0.0;
+    }
+    w = wave_sum(w);
+    wa = wave_sum(wa);
+    qa = wave_sum(qa);
+    if ((tid & 63) == 0) {
+        ss[0][tid >> 6] = w;
+        ss[1][tid >> 6] = wa;
+        ss[2][tid >> 6] = qa;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) b.resid[(size_t)s * b.chunks + ch] = ((ss[0] + ss[1]) + ss[2]) + ss[3];
+    if (tid == 0) {
+        double o[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) o[i] = (ss[i][0] + ss[i][1]) + (ss[i][2] + ss[i][3]);
+        b.rest[(size_t)s * b.rest_chunks + ch] = {o[0], o[1], o[2]};
+    }
 }
 
-// A workgroup of 16 waves per sequence.
-__global__ __launch_bounds__(1024) void verify_emit_kernel(VerifyBufs b, VerifyArgs v) {
-    __shared__ double sw[16];
-    __shared__ double s_before, s_target;
+// A workgroup of 4 waves per sequence.
+__global__ __launch_bounds__(256) void verify_emit_kernel(VerifyBufs b, VerifyArgs v) {
+    __shared__ double sw[4];
+    __shared__ double s_before, s_target, s_z;
     __shared__ int s_chunk, s_first, s_last;
     __shared__ bool s_whole;
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Decision d = decide<16>(b, v, s);
-    const bool drawn = d.t > 0.0f && d.z > 0.0;
+    const Decision d = b.dec[s];
     uint32_t token = (uint32_t)d.at;
-    if (drawn) {
-        Rest rest = rest_of(b, v, s, d);
+    if (d.t > 0.0f && d.z > 0.0f) {
+        const Rest r = rest_of(b, v, s, d);
         if (wave == 0) {
-            // the chunks' sums: of the rest, or (where the rest is p without one column) of p
-            const ChunkStat* st = b.stat + (size_t)d.row * b.chunks;
-            const double* rs = b.resid + (size_t)s * b.chunks;
-            const int out_chunk = rest.out < (uint32_t)b.cols ? (int)rest.out / b.chunk : -1;
+            const RestSum* rs = b.rest + (size_t)s * b.rest_chunks;
+            const double u = b.u[v.row[s] + d.drafts];
+            double z = 0.0, total = 0.0;
+            for (int c = lane; c < b.rest_chunks; c += 64) z += rs[c].w;
+            z = wave_sum(z);
             bool whole = false;  // the rest weighs nothing (by rounding): the token comes from p
             auto chunk_sum = [&](int c) {
-                if (rest.q && !whole) return rs[c];
-                const ChunkStat x = st[c];
-                double w = x.m == -INFINITY ? 0.0 : x.sum * weight(x.m, d.m, rest.inv_t);
-                if (c == out_chunk && !whole) w = __builtin_fmax(w - weight(rest.x[rest.out], d.m, rest.inv_t), 0.0);
-                return w;
+                const RestSum x = rs[c];
+                return whole ? x.w : r.q ? __builtin_fmax(__builtin_fma(-x.qa, z, x.wa), 0.0) : x.wa;
             };
-            double total = 0.0;
             for (int pass = 0; pass < 2; ++pass) {
                 total = 0.0;
-                for (int c = lane; c < b.chunks; c += 64) total += chunk_sum(c);
+                for (int c = lane; c < b.rest_chunks; c += 64) total += chunk_sum(c);
                 total = wave_sum(total);
-                if (total > 0.0 || whole) break;
+                if (total > 0.0) break;
                 whole = true;
             }
-            const double target = (double)b.u[v.row[s] + d.drafts] * total;
+            const double target = u * total;
             // the first chunk whose end exceeds the target; none (u >= 1 or not a number): the last that weighs
-            double before = 0.0, last_before = 0.0;
-            int found = -1, last = 0;
-            for (int c0 = 0; c0 < b.chunks && found < 0; c0 += 64) {
-                const double w = c0 + lane < b.chunks ? chunk_sum(c0 + lane) : 0.0;
+            double before = 0.0, pick_before = 0.0;
+            int chunk = 0;
+            bool found = false;
+            for (int c0 = 0; c0 < b.rest_chunks && !found; c0 += 64) {
+                const double w = c0 + lane < b.rest_chunks ? chunk_sum(c0 + lane) : 0.0;
                 double run = w;
 #pragma unroll
                 for (int off = 1; off < 64; off <<= 1) {
                     const double up = shfl_up64(run, off);
                     if (lane >= off) run += up;
                 }
-                const unsigned long long hit = __ballot(w > 0.0 && before + run > target);
-                const unsigned long long some = __ballot(w > 0.0);
-                const int pick = hit ? __ffsll(hit) - 1 : some ? 63 - __clzll(some) : -1;
-                if (pick >= 0) {
-                    const double start = before + shfl_up64(run, 1);
-                    const double at = __hiloint2double(__shfl(__double2hiint(start), pick, 64),
-                                                       __shfl(__double2loint(start), pick, 64));
-                    last = c0 + pick;
-                    last_before = pick == 0 ? before : at;
-                    if (hit) found = last;
+                const unsigned long long hit = __ballot(w > 0.0 && before + run > target), some = __ballot(w > 0.0);
+                const double up1 = shfl_up64(run, 1), start = lane ? up1 : 0.0;  // (every lane takes part in the shuffle)
+                if (some) {
+                    const int pick = hit ? __ffsll(hit) - 1 : 63 - __clzll(some);
+                    chunk = c0 + pick;
+                    pick_before = before + __hiloint2double(__shfl(__double2hiint(start), pick, 64),
+                                                            __shfl(__double2loint(start), pick, 64));
+                    found = hit != 0;
                 }
                 before += __hiloint2double(__shfl(__double2hiint(run), 63, 64), __shfl(__double2loint(run), 63, 64));
             }
             if (lane == 0) {
-                s_chunk = found >= 0 ? found : last;
-                s_before = last_before;
+                s_chunk = chunk;
+                s_before = pick_before;
                 s_target = target;
+                s_z = z;
                 s_whole = whole;
                 s_first = 0x7fffffff;
                 s_last = -1;
             }
         }
         __syncthreads();
-        if (s_whole) {
-            rest.q = nullptr;
-            rest.out = 0xffffffffu;
-        }
         // the chunk's columns, E to a thread, in order
-        const int E = b.chunk / 1024, c0 = s_chunk * b.chunk + tid * E;
-        double w[8], sum = 0.0;
+        constexpr int E = kRestChunk / 256;
+        const int c0 = s_chunk * kRestChunk + tid * E;
+        const double inv_t = 1.0 / (double)d.t, z = s_z;
+        const bool whole = s_whole;
+        float x[E], q[E];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            w[e] = e < E && c0 + e < b.cols ? rest(c0 + e) : 0.0;
+        for (int e = 0; e < E; ++e) {
+            x[e] = c0 + e < b.cols ? r.x[c0 + e] : -INFINITY;
+            q[e] = r.q && c0 + e < b.cols ? fmaxf(r.q[c0 + e], 0.0f) : 0.0f;
+        }
+        double w[E], sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            w[e] = weight(x[e], d.m, inv_t);
+            if (!whole) w[e] = r.q ? __builtin_fmax(w[e] - (double)q[e] * z, 0.0) : (uint32_t)(c0 + e) == r.out ? 0.0 : w[e];
             sum += w[e];
         }
         double run = sum;
@@ -390,7 +448,7 @@ __global__ __launch_bounds__(1024) void verify_emit_kernel(VerifyBufs b, VerifyA
         cum += run - sum;
         int first = 0x7fffffff, last = -1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < E; ++e) {
             cum += w[e];
             if (w[e] > 0.0) {
                 last = c0 + e;
@@ -404,7 +462,7 @@ __global__ __launch_bounds__(1024) void verify_emit_kernel(VerifyBufs b, VerifyA
         token = s_first != 0x7fffffff ? (uint32_t)s_first : s_last >= 0 ? (uint32_t)s_last : (uint32_t)d.at;
     }
     const uint32_t* y = b.drafts + (v.row[s] - s);
-    for (int i = tid; i < b.out_stride; i += 1024)
+    for (int i = tid; i < b.out_stride; i += 256)
         b.out[(size_t)s * b.out_stride + i] = i < d.accepted ? y[i] : i == d.accepted ? token : 0xffffffffu;
     if (tid == 0) b.accepted[s] = d.accepted;
 }
@@ -422,7 +480,9 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
     int e = 8;
     while (e > 1 && rows * ((cols + 1024 * e - 1) / (1024 * e)) < 1024) e /= 2;
     const int chunk = 1024 * e, chunks = (cols + chunk - 1) / chunk;
-    const size_t stat_bytes = sizeof(ChunkStat) * (size_t)rows * chunks, need = stat_bytes + 8 * (size_t)n * chunks;
+    const int rest_chunks = (cols + kRestChunk - 1) / kRestChunk;
+    const size_t stat_bytes = sizeof(ChunkStat) * (size_t)rows * chunks;
+    const size_t dec_bytes = sizeof(Decision) * (size_t)n, need = stat_bytes + dec_bytes + sizeof(RestSum) * (size_t)n * rest_chunks;
     if (need > ctx->verify_ws_bytes) {
         ZR_HIP(ctx, hipStreamSynchronize(ctx->stream));
         if (ctx->verify_ws) (void)hipFree(ctx->verify_ws);
@@ -456,7 +516,9 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
         b.probs = vb->d_draft_probs ? vb->d_draft_probs + draft0 * cols : nullptr;
         b.u = vb->d_uniforms + row0;
         b.stat = (ChunkStat*)ctx->verify_ws + row0 * chunks;
-        b.resid = (double*)((char*)ctx->verify_ws + stat_bytes) + (size_t)s0 * chunks;
+        b.dec = (Decision*)((char*)ctx->verify_ws + stat_bytes) + s0;
+        b.rest = (RestSum*)((char*)ctx->verify_ws + stat_bytes + dec_bytes) + (size_t)s0 * rest_chunks;
+        b.rest_chunks = rest_chunks;
         b.out = d_out + (size_t)s0 * out_stride;
         b.out_stride = out_stride;
         b.accepted = d_accepted + s0;
@@ -471,11 +533,12 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
             default: if (vec) stats(verify_stats_kernel<8, true>); else stats(verify_stats_kernel<8, false>); break;
         }
         ZR_LAUNCH_CHECK(ctx);
-        if (b.probs) {
-            hipLaunchKernelGGL(verify_residual_kernel, dim3(m * chunks), dim3(256), 0, ctx->stream, b, v);
-            ZR_LAUNCH_CHECK(ctx);
-        }
-        hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(1024), 0, ctx->stream, b, v);
+        if (vec && ((uintptr_t)vb->d_draft_probs & 15) == 0)
+            hipLaunchKernelGGL(verify_rest_kernel<true>, dim3(m * rest_chunks), dim3(256), 0, ctx->stream, b, v);
+        else
+            hipLaunchKernelGGL(verify_rest_kernel<false>, dim3(m * rest_chunks), dim3(256), 0, ctx->stream, b, v);
+        ZR_LAUNCH_CHECK(ctx);
+        hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(256), 0, ctx->stream, b, v);
         ZR_LAUNCH_CHECK(ctx);
         row0 += r;
         draft0 += r - m;

@@ -50,7 +50,7 @@ FUSED_KERNEL_STAGES = {
     "residual_mlp": ["rms_norm_vec_kernel", "rms_norm_kernel", "gemm_kernel", "gemm_swiglu_ksplit_kernel",
                      "splitk_reduce_kernel"],
     "device_sampling": ["argmax_partial_kernel", "argmax_final_kernel", "sample_kernel", "verify_stats_kernel",
-                        "verify_residual_kernel", "verify_emit_kernel"],
+                        "verify_rest_kernel", "verify_emit_kernel"],
 }
 
 
