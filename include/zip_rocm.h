@@ -119,7 +119,7 @@ uint64_t zr_kv_pool_bytes(const zr_context* ctx);
 /* Device address of the pool (NULL before zr_kv_pool_create; valid until the
  * pool is re-created or the context destroyed): [num_layers][n_pages][page
  * bytes], a page in the pool's own order, zr_kv_pool_bytes in all.  For
- * programs that move whole pages themselves (a peer copy, a checker). */
+ * programs that move whole pages themselves (a copy to another device). */
 void* zr_kv_pool_data(const zr_context* ctx);
 
 /* ------------------------------------------------------- microbatches --- */
@@ -406,8 +406,9 @@ zr_status zr_sample_last_logits(zr_context* ctx, int rows, const float* temperat
  * k): the accepted drafts, the drawn token, then 0xffffffff; d_accepted
  * [num_seqs]: the number accepted.  A logit that is not a number counts as -inf, a
  * draft outside the columns and a probability below 0 as probability 0; a row
- * without a finite logit gives token 0.  Weights and sums in f64, in a fixed
- * order.  cols <= 2^24.  The arrays marked host are read before the call
+ * without a finite logit gives token 0.  The drawn row's weights and sums are
+ * f64, the tests' sums f32 (1e-7 of themselves), all in a fixed order.
+ * cols <= 2^24.  The arrays marked host are read before the call
  * returns; zr_verify_async enqueues the rest on the context stream.  No
  * counterpart in the reference (one token a step). */
 typedef struct {
@@ -422,6 +423,17 @@ zr_status zr_verify(zr_context* ctx, const float* d_logits, int cols, const zr_v
                     uint32_t* d_out_tokens, int out_stride, int* d_accepted);
 zr_status zr_verify_async(zr_context* ctx, const float* d_logits, int cols, const zr_verify_batch* vb,
                           uint32_t* d_out_tokens, int out_stride, int* d_accepted);
+/* A forward whose every row is verified: sequence s brings q_len[s] = k + 1
+ * tokens, the last one emitted and k drafts after it (k <= 255), all of which are
+ * appended to its cache rows; the LM head runs over all rows and zr_verify over its
+ * logits.  temperature host [num_seqs], uniforms host [sum q_len], d_draft_probs
+ * device [sum k, vocab] (complete before the call) or NULL, out_tokens and accepted
+ * host, as zr_verify's.  The rows of drafts that were not accepted are the caller's
+ * to drop.  At most 2^29 logits a call.  zr_sample_last_logits is refused until the
+ * next forward (this one keeps no last rows' logits). */
+zr_status zr_forward_verify(zr_context* ctx, const zr_microbatch* mb, const float* temperature,
+                            const float* uniforms, const float* d_draft_probs, uint32_t* out_tokens,
+                            int out_stride, int* accepted);
 /* y = rms_norm(x) * gamma (tensor_ops.rs:285-304), device f32 [rows, cols]. */
 zr_status zr_rms_norm(zr_context* ctx, const float* d_x, const float* d_gamma, float* d_y, int rows,
                       int cols);

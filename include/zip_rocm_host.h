@@ -139,6 +139,17 @@ zr_status zrh_fork(const zrh_backend* parent, zrh_backend* child);
  * position back by as many; pages left empty stay bound to the session.  More
  * rows than the window holds: ZR_E_INVALID, nothing dropped. */
 zr_status zrh_truncate(zrh_backend* b, int drop_rows);
+/* One verified step of n sessions (zr_forward_verify): session i takes
+ * draft_len[i] + 1 of `tokens`, its last emitted token and the drafts after it,
+ * and emits its accepted drafts and one token more.  Its window then ends behind
+ * the last accepted draft (the other rows are dropped as by zrh_truncate) and its
+ * position has moved by accepted + 1: the next step's first token is the last one
+ * emitted here.  Refused, with nothing changed, where the drafted rows would slide
+ * a session's window (rows that a rejection could not bring back): bring fewer
+ * drafts, or none.  On an error every session is as before. */
+zr_status zrh_verify_batch(zrh_backend* const* backends, int n, const int* draft_len, const uint32_t* tokens,
+                           const float* temperature, const float* uniforms, const float* d_draft_probs,
+                           uint32_t* out_tokens, int out_stride, int* accepted);
 /* Pages bound to the session but outside its window (after a trim, a clear or
  * a truncation) go back to the pool; *released (nullable) is their number. */
 zr_status zrh_release_idle_pages(zrh_backend* b, int* released);

@@ -7,11 +7,11 @@ interface (mesh_amd.provider).
 from .provider import (BackendMicrobatchExecutor, DecodeMicrobatchOutput, DecodeMicrobatchRequest,
                        DecodePipeline, DeviceBuffer, DeviceContext, ExecutionProviderKind, FastPathPlanner, KVCacheBlob,
                        KVCacheSnapshot, KVCacheWireSnapshot, KVSequenceState, KVTransfer, ModelGeometry,
-                       RocmExecutionBackend,
+                       RocmExecutionBackend, VerifyMicrobatchOutput, VerifyMicrobatchRequest,
                        bf16_bits, device_info, executor_contract, probe_provider, verify_device)
 
 __all__ = ["BackendMicrobatchExecutor", "DecodeMicrobatchOutput", "DecodeMicrobatchRequest", "DecodePipeline",
            "DeviceBuffer",
            "DeviceContext", "ExecutionProviderKind", "FastPathPlanner", "KVCacheBlob", "KVCacheSnapshot",
-           "KVCacheWireSnapshot", "KVSequenceState", "KVTransfer", "ModelGeometry", "RocmExecutionBackend", "bf16_bits",
-           "device_info", "executor_contract", "probe_provider", "verify_device"]
+           "KVCacheWireSnapshot", "KVSequenceState", "KVTransfer", "ModelGeometry", "RocmExecutionBackend",
+           "VerifyMicrobatchOutput", "VerifyMicrobatchRequest", "bf16_bits", "device_info", "executor_contract", "probe_provider", "verify_device"]

@@ -172,6 +172,8 @@ SIGNATURES = [
     ("zr_verify", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(VerifyBatch), C.c_void_p, C.c_int, C.c_void_p]),
     ("zr_verify_async", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(VerifyBatch), C.c_void_p, C.c_int,
                                   C.c_void_p]),
+    ("zr_forward_verify", C.c_int, [C.c_void_p, C.POINTER(Microbatch), c_f32_p, c_f32_p, C.c_void_p, c_u32_p, C.c_int,
+                                    c_int_p]),
     ("zr_rms_norm", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
     ("zr_gemm", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]),
     ("zr_gemm_swiglu", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]),
@@ -217,6 +219,8 @@ SIGNATURES = [
     ("zrh_release_pages", C.c_int, [C.c_void_p]),
     ("zrh_fork", C.c_int, [C.c_void_p, C.c_void_p]),
     ("zrh_truncate", C.c_int, [C.c_void_p, C.c_int]),
+    ("zrh_verify_batch", C.c_int, [c_void_pp, C.c_int, c_int_p, c_u32_p, c_f32_p, c_f32_p, C.c_void_p, c_u32_p, C.c_int,
+                                   c_int_p]),
     ("zrh_release_idle_pages", C.c_int, [C.c_void_p, c_int_p]),
     ("zrh_pool_compact", C.c_int, [C.c_void_p, c_int_p]),
     ("zrh_pool_shared_pages", C.c_int, [C.c_void_p]),

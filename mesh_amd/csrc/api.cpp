@@ -136,10 +136,11 @@ static void free_ctx_buffers(zr_context* ctx) {
     void* bufs[] = {ctx->hidden, ctx->hidden2, ctx->xa, ctx->qkv, ctx->q_rope, ctx->attn_a, ctx->proj, ctx->ffn_a,
                     ctx->logits, ctx->final_a, ctx->tokens_out, ctx->splitk_ws, ctx->attn_part,
                     ctx->argmax_ws, ctx->inv_freq, ctx->kv_pool, ctx->embedding, ctx->lm_head,
-                    ctx->final_norm, ctx->d_token_err};
+                    ctx->final_norm, ctx->d_token_err, ctx->row_logits, ctx->row_splitk, ctx->verify_io};
     for (void* b : bufs)
         if (b) hipFree(b);
     if (ctx->h_token_err) hipHostFree(ctx->h_token_err);
+    if (ctx->verify_io_host) hipHostFree(ctx->verify_io_host);
     for (auto& L : ctx->layers) {
         void* lb[] = {L.w_qkv, L.w_o, L.w_gate_up, L.w_down, L.attn_norm, L.mlp_norm};
         for (void* b : lb)
@@ -768,7 +769,7 @@ static zr_status check_ready(zr_context* ctx) {
 }
 
 static zr_status run_forward(zr_context* ctx, StagedMeta* st, const uint32_t* d_tokens, uint32_t* d_out_tokens,
-                             float* d_out_logits, float* h_partials, bool waits) {
+                             float* d_out_logits, float* h_partials, bool waits, bool all_rows = false) {
     zr_status rc = check_ready(ctx);
     if (rc) return rc;
     const zr_model_desc& d = ctx->desc;
@@ -838,6 +839,13 @@ static zr_status run_forward(zr_context* ctx, StagedMeta* st, const uint32_t* d_
             ZR_HIP(ctx, hipMemcpyAsync(h_partials + ((size_t)l * 2 + 1) * T * H, ctx->proj, sizeof(float) * T * H,
                                        hipMemcpyDeviceToHost, ctx->stream));
     }
+    if (all_rows) {  // the LM head over every row, into row_logits
+        if ((rc = launch_rms_norm(ctx, hidden, down, hidden, ctx->final_norm, nullptr, ctx->xa, lo, nullptr, T, H)))
+            return rc;
+        ctx->last_logits = false;
+        return launch_gemm(ctx, ctx->xa, ctx->lm_head, ctx->row_logits, nullptr, T, d.vocab, H, kEpiStore);
+    }
+    ctx->last_logits = true;
     // final residual + norm on the last row of every sequence, LM head, argmax
     if ((rc = launch_rms_norm(ctx, hidden, down, hidden, ctx->final_norm, nullptr, ctx->final_a, lo,
                               st->last_rows, S, H)))
@@ -1285,6 +1293,7 @@ zr_status zr_graph_launch(zr_context* ctx, zr_graph* g) {
     if (zr_status rc = pages_current(ctx, g->page_epoch)) return rc;
     ZR_HIP(ctx, hipGraphLaunch(g->exec, ctx->stream));
     if (g->token_check) ctx->token_check_pending = true;
+    ctx->last_logits = true;
     return ZR_OK;
 }
 
@@ -1500,6 +1509,7 @@ zr_status zr_step_graph_launch(zr_step_graph* g, const zr_microbatch* mb, const 
     ZR_HIP(ctx, hipGraphLaunch(exec, ctx->stream));
     ZR_HIP(ctx, hipEventRecord(g->replayed[b], ctx->stream));
     g->replay_pending[b] = true;
+    ctx->last_logits = true;
     ctx->token_check_pending = true;  // the replay copies the id-check word (device-fed ids)
     if (h_out_tokens)
         ZR_HIP(ctx, hipMemcpyAsync(h_out_tokens, d_out_tokens, 4 * (size_t)mb->num_seqs, hipMemcpyDeviceToHost,
@@ -2140,6 +2150,7 @@ zr_status zr_sample_last_logits(zr_context* ctx, int rows, const float* temperat
                                 const uint64_t* seeds, uint32_t* out_tokens) {
     if (!ctx || !out_tokens) return set_global_err(ZR_E_INVALID, "null argument");
     if (!ctx->logits || !ctx->tokens_out) return set_err(ctx, ZR_E_INVALID, "no logits to sample");
+    if (!ctx->last_logits) return set_err(ctx, ZR_E_INVALID, "the last forward was a verification: it left no last rows' logits");
     if (rows <= 0 || rows > ctx->desc.max_seqs)
         return set_err(ctx, ZR_E_INVALID, "Device sampling received %d rows", rows);
     zr_status rc = launch_sample(ctx, ctx->logits, rows, ctx->desc.vocab, temperature, top_p, seeds, ctx->tokens_out);
@@ -2183,6 +2194,80 @@ zr_status zr_verify(zr_context* ctx, const float* d_logits, int cols, const zr_v
     zr_status rc = zr_verify_async(ctx, d_logits, cols, vb, d_out_tokens, out_stride, d_accepted);
     if (!rc) ZR_HIP(ctx, hipStreamSynchronize(ctx->stream));
     return rc;
+}
+
+// Device memory of at least `need` bytes; what the old one held is lost.
+static zr_status grow(zr_context* ctx, void** p, size_t* have, size_t need, const char* what) {
+    if (need <= *have) return ZR_OK;
+    ZR_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    if (*p) (void)hipFree(*p);
+    *p = nullptr;
+    *have = 0;
+    const hipError_t e = hipMalloc(p, need);
+    if (e != hipSuccess)
+        return set_err(ctx, e == hipErrorOutOfMemory ? ZR_E_OOM : ZR_E_HIP, "%s of %zu bytes: %s", what, need,
+                       hipGetErrorString(e));
+    *have = need;
+    return ZR_OK;
+}
+
+zr_status zr_forward_verify(zr_context* ctx, const zr_microbatch* mb, const float* temperature, const float* uniforms,
+                            const float* d_draft_probs, uint32_t* out_tokens, int out_stride, int* accepted) {
+    if (!ctx || !mb) return set_global_err(ZR_E_INVALID, "null argument");
+    if (!mb->tokens || !mb->q_len || !temperature || !uniforms || !out_tokens || !accepted)
+        return set_err(ctx, ZR_E_INVALID, "null argument");
+    ZR_HIP(ctx, hipSetDevice(ctx->device));
+    const int n = mb->num_seqs, V = ctx->desc.vocab;
+    StagedMeta* st = ctx->scratch_stage;
+    if (zr_status rc = stage_microbatch(ctx, mb, st)) return rc;  // (checks the counts, the rows and the token ids)
+    const int T = st->total_q;
+    if ((size_t)T * V > (size_t)1 << 29)
+        return set_err(ctx, ZR_E_INVALID, "verification of %d rows of %d logits: at most 2^29 logits a call", T, V);
+    if (zr_status rc = check_ready(ctx)) return rc;
+    std::vector<int> lens(n);
+    for (int s = 0; s < n; ++s) lens[s] = mb->q_len[s] - 1;
+    // uniforms [T], drafts [T - n] to the device; tokens [n][out_stride], accepted [n] back
+    const size_t in = (size_t)T + (T - n), out = (size_t)n * std::max(out_stride, 0) + n;
+    if (zr_status rc = grow(ctx, &ctx->verify_io, &ctx->verify_io_bytes, 4 * (in + out), "verification staging")) return rc;
+    if (4 * (in + out) > ctx->verify_io_host_bytes) {
+        if (ctx->verify_io_host) (void)hipHostFree(ctx->verify_io_host);
+        ctx->verify_io_host = nullptr;
+        ctx->verify_io_host_bytes = 0;
+        ZR_HIP(ctx, hipHostMalloc(&ctx->verify_io_host, 4 * (in + out), hipHostMallocDefault));
+        ctx->verify_io_host_bytes = 4 * (in + out);
+    }
+    uint32_t* h = (uint32_t*)ctx->verify_io_host;
+    uint32_t* d = (uint32_t*)ctx->verify_io;
+    zr_verify_batch vb{n, lens.data(), d + T, d_draft_probs, temperature, (const float*)d};
+    if (zr_status rc = verify_check(ctx, ctx->verify_io, V, &vb, out_tokens, out_stride, accepted)) return rc;
+    if (zr_status rc = grow(ctx, (void**)&ctx->row_logits, &ctx->row_logits_bytes, (size_t)4 * T * V, "verification logits"))
+        return rc;
+    const size_t splitk = gemm_ws_floats(T, V, ctx->desc.hidden, kEpiStore);
+    if (splitk > ctx->splitk_ws_floats)
+        if (zr_status rc = grow(ctx, (void**)&ctx->row_splitk, &ctx->row_splitk_bytes, 4 * splitk, "split-K workspace")) return rc;
+    memcpy(h, uniforms, 4 * (size_t)T);
+    for (int s = 0, row = 0; s < n; row += mb->q_len[s], ++s) memcpy(h + T + row - s, mb->tokens + row + 1, 4 * (size_t)lens[s]);
+    ZR_HIP(ctx, hipMemcpyAsync(d, h, 4 * in, hipMemcpyHostToDevice, ctx->stream));
+    // the LM head over all rows may split further than that over last rows
+    float* const ws = ctx->splitk_ws;
+    const size_t ws_floats = ctx->splitk_ws_floats;
+    if (splitk > ws_floats) {
+        ctx->splitk_ws = ctx->row_splitk;
+        ctx->splitk_ws_floats = ctx->row_splitk_bytes / 4;
+    }
+    zr_status rc = run_forward(ctx, st, nullptr, nullptr, nullptr, nullptr, true, true);
+    ctx->splitk_ws = ws;
+    ctx->splitk_ws_floats = ws_floats;
+    if (!rc) rc = launch_verify(ctx, ctx->row_logits, V, &vb, d + in, out_stride, (int*)(d + in + (size_t)n * out_stride));
+    hipError_t e = hipSuccess;
+    if (!rc) e = hipMemcpyAsync(h + in, d + in, 4 * out, hipMemcpyDeviceToHost, ctx->stream);
+    const hipError_t w = hipStreamSynchronize(ctx->stream);
+    if (e == hipSuccess) e = w;
+    if (!rc && e != hipSuccess) rc = set_err(ctx, ZR_E_HIP, "forward: %s", hipGetErrorString(e));
+    if (rc) return rc;
+    memcpy(out_tokens, h + in, 4 * (size_t)n * out_stride);
+    memcpy(accepted, h + in + (size_t)n * out_stride, 4 * (size_t)n);
+    return ZR_OK;
 }
 
 zr_status zr_rms_norm(zr_context* ctx, const float* d_x, const float* d_gamma, float* d_y, int rows, int cols) {

@@ -931,6 +931,42 @@ zr_status zrh_truncate(zrh_backend* b, int drop_rows) {
     return ZR_OK;
 }
 
+zr_status zrh_verify_batch(zrh_backend* const* backends, int n, const int* draft_len, const uint32_t* tokens,
+                           const float* temperature, const float* uniforms, const float* d_draft_probs,
+                           uint32_t* out_tokens, int out_stride, int* accepted) {
+    if (!backends || !draft_len || !tokens || !temperature || !uniforms || !out_tokens || !accepted || n <= 0)
+        return set_global_err(ZR_E_INVALID, "null argument");
+    std::vector<int> q_len(n);
+    for (int i = 0; i < n; ++i) {
+        if (!backends[i]) return set_global_err(ZR_E_INVALID, "null backend");
+        zr_context* ctx = backends[i]->ctx;
+        if (draft_len[i] < 0 || draft_len[i] > 255)
+            return set_err(ctx, ZR_E_INVALID, "session %d has %d drafts (0..255)", i, draft_len[i]);
+        if (out_stride <= draft_len[i])
+            return set_err(ctx, ZR_E_INVALID, "output stride %d for %d drafts and a token", out_stride, draft_len[i]);
+        const int window = std::max(backends[i]->max_seq_len, 1);
+        if (draft_len[i] > 0 && backends[i]->kv.seq_len + draft_len[i] + 1 > window)
+            return set_err(ctx, ZR_E_INVALID, "session %d: %d drafts behind %d rows would slide its %d-token window", i,
+                           draft_len[i], backends[i]->kv.seq_len, window);
+        q_len[i] = draft_len[i] + 1;
+    }
+    PoolTxn txn(backends[0]->pool);
+    Assembled a;
+    Saved saved;
+    zr_status rc = assemble(backends, n, q_len.data(), true, a, saved, txn);
+    if (rc) return rc;
+    if (!backends[0]->ctx) rc = set_global_err(ZR_E_INVALID, "bookkeeping-only pool has no device context");
+    zr_microbatch mb = as_microbatch(a, tokens);
+    if (!rc)
+        rc = zr_forward_verify(backends[0]->ctx, &mb, temperature, uniforms, d_draft_probs, out_tokens, out_stride, accepted);
+    for (int i = 0; i < n && !rc; ++i) {
+        backends[i]->position += q_len[i];
+        rc = zrh_truncate(backends[i], draft_len[i] - accepted[i]);
+    }
+    if (rc) saved.restore(backends, n, txn);
+    return rc;
+}
+
 zr_status zrh_release_idle_pages(zrh_backend* b, int* released) {
     if (!b) return set_global_err(ZR_E_INVALID, "null backend");
     SessionKV& kv = b->kv;

@@ -213,6 +213,15 @@ struct zr_context {
     uint16_t* ffn_a = nullptr;   // SwiGLU output, A of down
     uint16_t* final_a = nullptr; // [S, H] normed last rows, A of the LM head
     float* logits = nullptr;     // [S, V]
+    bool last_logits = true;     // the last forward left logits there (a verification's are in row_logits)
+    float* row_logits = nullptr; // [T, V] of a verification, grown as asked for
+    size_t row_logits_bytes = 0;
+    float* row_splitk = nullptr; // split-K workspace of its LM head, where splitk_ws is too small
+    size_t row_splitk_bytes = 0;
+    void* verify_io = nullptr;   // its uniforms, drafts and results, and their pinned copy
+    size_t verify_io_bytes = 0;
+    void* verify_io_host = nullptr;
+    size_t verify_io_host_bytes = 0;
     uint32_t* tokens_out = nullptr; // [S]
     float* splitk_ws = nullptr;     // split-K partial workspace
     size_t splitk_ws_floats = 0;

@@ -798,6 +798,26 @@ class DecodeMicrobatchOutput:
     execution_time_ms: int
 
 
+@dataclass
+class VerifyMicrobatchRequest:
+    """One session of a verified step: its last emitted token and the drafts after it."""
+    session_id: str
+    token: int
+    drafts: Sequence[int]
+    backend: RocmExecutionBackend
+    job_id: str = ""
+    temperature: float = 0.0
+    uniforms: Optional[Sequence[float]] = None  # len(drafts) + 1 in [0, 1), where the temperature is above 0
+
+
+@dataclass
+class VerifyMicrobatchOutput:
+    session_id: str
+    tokens: List[int]  # the accepted drafts and the token after them
+    accepted: int
+    execution_time_ms: int
+
+
 def _backend_array(backends):
     arr = (C.c_void_p * len(backends))(*[b.h for b in backends])
     return C.cast(arr, C.POINTER(C.c_void_p)), arr
@@ -888,6 +908,55 @@ class BackendMicrobatchExecutor:
                                                     lg, pa))
         ms = int((time.perf_counter() - t0) * 1000)
         return [DecodeMicrobatchOutput(r.session_id, logits[i] if logits is not None else None, int(out_tokens[i]), ms)
+                for i, r in enumerate(requests)]
+
+    @staticmethod
+    def verify_batch(requests: List[VerifyMicrobatchRequest], draft_probs=None) -> List[VerifyMicrobatchOutput]:
+        """One verified step of every session in one microbatch (zrh_verify_batch):
+        emits each session's accepted drafts and one token more, and leaves its window
+        behind the last accepted draft.  draft_probs: the drafts' distributions
+        [sum of drafts, vocab] (an array, or a DeviceBuffer of f32 that is complete),
+        None for drafts that were certain (looked up, or greedy)."""
+        if not requests:
+            raise ZrError(-1, "Decode microbatch requires at least one backend and token")
+        ctx = requests[0].backend.ctx
+        for r in requests:
+            if r.backend.ctx is not ctx:
+                raise ZrError(-1, "Fast-path decode batch requires one shared model residency")
+            if r.uniforms is None and r.temperature > 0.0:
+                raise ZrError(-1, f"session {r.session_id}: a temperature above 0 needs uniforms")
+            if r.uniforms is not None and len(r.uniforms) != len(r.drafts) + 1:
+                raise ZrError(-1, f"session {r.session_id}: {len(r.uniforms)} uniforms for {len(r.drafts)} drafts and a token")
+        n = len(requests)
+        lens = np.ascontiguousarray([len(r.drafts) for r in requests], np.int32)
+        toks = np.ascontiguousarray([t for r in requests for t in (r.token, *r.drafts)], np.uint32)
+        temps = np.ascontiguousarray([r.temperature for r in requests], np.float32)
+        u = np.zeros(toks.size, np.float32) if all(r.uniforms is None for r in requests) else np.ascontiguousarray(
+            [x for r in requests for x in (r.uniforms if r.uniforms is not None else [0.0] * (len(r.drafts) + 1))], np.float32)
+        q = owned = None
+        if draft_probs is not None and lens.any():
+            size = 4 * int(lens.sum()) * ctx.geo.vocab
+            if not isinstance(draft_probs, DeviceBuffer):
+                draft_probs = np.ascontiguousarray(draft_probs, np.float32)
+            if draft_probs.nbytes < size or (isinstance(draft_probs, np.ndarray) and draft_probs.nbytes != size):
+                raise ZrError(-1, f"draft probabilities of {draft_probs.nbytes} bytes for {int(lens.sum())} drafts of "
+                                  f"{ctx.geo.vocab} columns")
+            q = draft_probs
+            if isinstance(q, np.ndarray):
+                q = owned = DeviceBuffer.from_numpy(ctx, q)
+        stride = int(lens.max()) + 1
+        out, acc = np.zeros((n, stride), np.uint32), np.zeros(n, np.int32)
+        ptrs, _keep = _backend_array([r.backend for r in requests])
+        t0 = time.perf_counter()
+        try:
+            ctx.check(ctx.lib.zrh_verify_batch(ptrs, n, _ptr(lens, C.c_int), _ptr(toks, C.c_uint32), _ptr(temps, C.c_float),
+                                               _ptr(u, C.c_float), q.ptr if q is not None else None, _ptr(out, C.c_uint32),
+                                               stride, _ptr(acc, C.c_int)))
+        finally:
+            if owned is not None:
+                owned.free()
+        ms = int((time.perf_counter() - t0) * 1000)
+        return [VerifyMicrobatchOutput(r.session_id, out[i, :acc[i] + 1].tolist(), int(acc[i]), ms)
                 for i, r in enumerate(requests)]
 
     @staticmethod

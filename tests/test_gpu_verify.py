@@ -1,7 +1,8 @@
 """Draft verification against a restatement of its definition in 64 bits, row by
-row.  Tokens and counts are whole numbers and have to be equal: weights and sums
-are held in f64 on both sides, and random uniforms come no nearer to a border
-than their 2^-24 steps allow by chance (about 1e-9 a token)."""
+row.  Tokens and counts are whole numbers and have to be equal: the drawn row's
+weights and sums are held in f64 on both sides, so a random uniform meets a border
+between two tokens with a chance of about 1e-9; a draft's test has one border, and
+sums Z in f32 (a few 2^-24 of themselves) move it by 1e-6 of a probability at most."""
 import ctypes as C
 
 import numpy as np
