@@ -200,7 +200,11 @@ static BlobLayout blob_layout(int S, int stride, int total_q, int n_items, int n
 
 void stage_fixed_bytes(const zr_context* ctx, int S, int total_q, const StageFixed& f, size_t* host_bytes,
                        size_t* dev_bytes) {
-    const BlobLayout b = blob_layout(S, f.stride, total_q, f.items_cap, f.merge_cap, 0, ctx->head_dim);
+    SharedCounts sh;
+    sh.units = f.units_cap;
+    sh.merges = f.smerge_cap;
+    sh.sources = f.ssrc_cap;
+    const BlobLayout b = blob_layout(S, f.stride, total_q, f.items_cap, f.merge_cap, 0, ctx->head_dim, sh);
     *host_bytes = b.host_bytes;
     *dev_bytes = b.total_bytes;
 }
@@ -401,7 +405,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     std::vector<SharedSegment> segments;
     std::vector<int> cover(S, 0);
     const char* shared_env = getenv("ZR_SHARED_PREFIX");
-    if (qpt > 0 && S > 1 && !fixed && !(shared_env && atoi(shared_env) == 0)) {
+    if (qpt > 0 && S > 1 && !(shared_env && atoi(shared_env) == 0)) {
         std::vector<char> takes(S);
         for (int s = 0; s < S; ++s) takes[s] = !as_prefill(s);
         shared_segments(mb, takes, &segments, &cover);
@@ -652,14 +656,22 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     if (const char* env = getenv("ZR_ATTN_FUSE_ROPE")) st->fuse_rope = may_fuse && atoi(env) != 0;
     st->grid_items = st->n_attn_items;
     st->grid_merge = st->n_merge;
+    st->grid_units = st->n_sunits;
+    st->grid_smerge = st->n_smerge;
     if (fixed) {
         if (!st->pure_decode || st->n_pblocks > 0) return no_fit("not a decode step of one row per sequence");
         if (fixed->plan_only) return ZR_OK;
         if (st->n_attn_items > fixed->items_cap) return no_fit("attention items");
         if (st->n_merge > fixed->merge_cap) return no_fit("split merges");
-        st->fuse_rope = fixed->fuse_rope;
+        if ((st->n_sunits > 0) != (fixed->units_cap > 0) || st->n_sunits > fixed->units_cap ||
+            st->n_smerge > fixed->smerge_cap || (int)st->h_ssrc.size() > fixed->ssrc_cap ||
+            (st->n_sunits > 0 && (st->unit_cols != fixed->unit_cols || st->merge_wide != fixed->merge_wide)))
+            return no_fit("shared segments");
+        st->fuse_rope = fixed->fuse_rope && st->n_sunits == 0;
         st->grid_items = fixed->items_cap;
         st->grid_merge = fixed->merge_cap;
+        st->grid_units = fixed->units_cap;
+        st->grid_smerge = fixed->smerge_cap;
     }
 
     const size_t need_part = (size_t)st->n_part_items * ctx->local_kv_heads * 16 * (ctx->head_dim + 2);
@@ -676,9 +688,9 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
 
     // one blob: inputs, derived arrays, attention items
     SharedCounts sh;
-    sh.units = st->n_sunits;
-    sh.merges = st->n_smerge;
-    sh.sources = (int)st->h_ssrc.size();
+    sh.units = st->grid_units;
+    sh.merges = st->grid_smerge;
+    sh.sources = fixed ? fixed->ssrc_cap : (int)st->h_ssrc.size();
     const BlobLayout L = blob_layout(S, blob_stride, total_q, st->grid_items, st->grid_merge, st->n_pblocks,
                                      ctx->head_dim, sh);
     const size_t host_bytes = L.host_bytes, total_bytes = L.total_bytes;
@@ -729,6 +741,9 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
         memcpy(hb + L.o_sunit, st->h_sunits.data(), 4 * st->h_sunits.size());
         memcpy(hb + L.o_smrg, st->h_smerge.data(), 16 * st->h_smerge.size());
         memcpy(hb + L.o_ssrc, st->h_ssrc.data(), 16 * st->h_ssrc.size());
+        // empty records (no rows, no sources): their workgroups return at once
+        for (int i = st->n_sunits; i < st->grid_units; ++i) memset(hb + L.o_sunit + 4 * (size_t)kUnitInts * i, 0, 4 * kUnitPages);
+        memset(hb + L.o_smrg + 16 * (size_t)st->n_smerge, 0, 16 * (size_t)(st->grid_smerge - st->n_smerge));
     }
     unsigned char* db = (unsigned char*)st->dev;
     st->sunits = (int*)(db + L.o_sunit);
@@ -1361,8 +1376,9 @@ zr_status step_graph_quiesce(zr_step_graph* g) {
 }
 
 // Sizes a bucket for the sequence count and the counts of `mb` with room to
-// grow: records for 1.25x the step's attention items (+64) and merges (+16),
-// the context's widest block table, and the step's RoPE placement.
+// grow: records for 1.25x the step's attention items (+64), merges (+16) and
+// units of shared segments (+8), the context's widest block table, and the step's
+// RoPE placement.
 zr_status step_graph_setup(zr_step_graph* g, const zr_microbatch* mb) {
     zr_context* ctx = g->ctx;
     StagedMeta probe;
@@ -1381,7 +1397,17 @@ zr_status step_graph_setup(zr_step_graph* g, const zr_microbatch* mb) {
     f.merge_cap = probe.n_merge + std::max(16, probe.n_merge / 4);
     f.fuse_rope = probe.fuse_rope;
     // partials of every item a step of the bucket can hold (decode items only)
-    const size_t need_part = (size_t)f.items_cap * ctx->local_kv_heads * 16 * (ctx->head_dim + 2);
+    if (probe.n_sunits > 0) {
+        f.units_cap = probe.n_sunits + std::max(8, probe.n_sunits / 4);
+        f.smerge_cap = probe.n_smerge;  // every row of a decode step
+        f.ssrc_cap = (int)probe.h_ssrc.size() + std::max(16, (int)probe.h_ssrc.size() / 4);
+        f.unit_cols = probe.unit_cols;
+        f.merge_wide = probe.merge_wide;
+    }
+    // ... and of the units' 16-column groups behind them
+    const int group_items = probe.n_part_items - probe.n_attn_items;
+    const size_t need_part = (size_t)(f.items_cap + group_items + group_items / 4) * ctx->local_kv_heads * 16 *
+                             (ctx->head_dim + 2);
     if (need_part > ctx->attn_part_floats) {
         if (ctx->attn_part) hipFree(ctx->attn_part);
         ++ctx->buffer_epoch;

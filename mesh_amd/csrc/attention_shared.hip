@@ -950,7 +950,7 @@ zr_status launch_shared_attention(zr_context* ctx, StagedMeta* st, int layer, co
     a.stride = st->stride;
     a.units = st->sunits;
     a.rec = st->attn_rec;
-    a.n_units = st->n_sunits;
+    a.n_units = st->grid_units;
     a.n_tails = st->grid_items;
     a.kv_heads = ctx->local_kv_heads;
     a.unit_groups = (a.n_units * a.kv_heads + 7) / 8;
@@ -967,9 +967,9 @@ zr_status launch_shared_attention(zr_context* ctx, StagedMeta* st, int layer, co
 }
 
 zr_status launch_shared_merge(zr_context* ctx, StagedMeta* st, float* out, uint16_t* out_bf16) {
-    if (st->n_smerge == 0) return ZR_OK;
+    if (st->grid_smerge == 0) return ZR_OK;
     const size_t lo = (ctx->desc.flags & ZR_FLAG_SPLIT_ACTIVATIONS) ? a_plane(st->total_q, ctx->q_cols) : 0;
-    const int jobs = st->n_smerge * ctx->local_q_heads;
+    const int jobs = st->grid_smerge * ctx->local_q_heads;
     const bool wide = st->merge_wide;
     auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(wide ? jobs : (jobs + 3) / 4), dim3(256), 0, ctx->stream, ctx->attn_part,

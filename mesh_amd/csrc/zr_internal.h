@@ -341,6 +341,7 @@ struct StagedMeta {
     int grid_items = 0;       // decode attention records the launch covers (n_attn_items, or a bucket's
                               // capacity whose records past n_attn_items are empty)
     int grid_merge = 0;       // merge records the launch covers (likewise)
+    int grid_units = 0, grid_smerge = 0;  // shared units and merged rows (likewise)
     // one device allocation holding every array below
     void* dev = nullptr;
     size_t dev_bytes = 0, cap_bytes = 0;
@@ -404,6 +405,10 @@ struct StageFixed {
     int items_cap = 0;               // decode attention records
     int merge_cap = 0;               // merge records
     bool fuse_rope = false;          // RoPE + KV append inside attention (fixed per bucket)
+    // shared segments (units_cap 0: none); their unit width and merge form are fixed per bucket
+    int units_cap = 0, smerge_cap = 0, ssrc_cap = 0;
+    int unit_cols = 128;
+    bool merge_wide = false;
     unsigned char* host = nullptr;
     size_t host_cap = 0;
     void* dev = nullptr;
