@@ -40,7 +40,6 @@ namespace {
 constexpr int kSeqs = 256;        // sequences a launch (their lengths and temperatures are kernel arguments)
 constexpr int kMaxDrafts = 255;   // drafts of one sequence
 constexpr int kRestChunk = 2048;  // columns of an emission row's chunk
-constexpr double kNothing = -1000.0;  // exp of it is 0
 constexpr float kLog2E = 1.44269504088896341f;
 
 struct VerifyArgs {
@@ -74,57 +73,87 @@ struct RestSum {
     double w, wa, qa;  // sum of w; over the columns with w > q Z: of w and of q
 };
 
-// What the tests of a sequence come to.
+// What the tests of a sequence come to: where its token is drawn from.
 struct Decision {
-    int drafts, accepted, row;  // drafts of the sequence; accepted ones; the row the token comes from
-    float m;                    // ... its largest logit
-    int at;                     // ... the first place of it
-    float z;                    // ... the f32 sum of its weights (0: none weighs)
+    float m;       // the row's largest logit
+    int at;        // the first place of it
+    float z;       // the f32 sum of its weights (0: none weighs)
     float t;
-    int pad;
+    int row;       // of the logits
+    int probs;     // ... of the rejected draft's probabilities, or -1: p ...
+    uint32_t out;  // ... without a certain draft's own column (none: 0xffffffff)
+    float u;
+    int drafts, accepted;
 };
 
-// exp(y) for y <= 0: y = k ln 2 + r, |r| <= ln 2 / 2 (k by adding and taking away
-// 1.5 2^52, which leaves it in the sum's low bits; ln 2 in two parts, Cody and
-// Waite's, k times the first exact), and the Taylor series of exp(r) to r^10 (the
-// next term is below 2.2e-13).  0 below -700.
-__device__ inline double exp_neg(double y) {
-    constexpr double kRound = 6755399441055744.0;
-    const double t = __builtin_fma(y, 1.4426950408889634074, kRound), k = t - kRound;
-    double r = __builtin_fma(-k, 0.693147180369123816490, y);
-    r = __builtin_fma(-k, 1.90821492927058770002e-10, r);
-    double e = 1.0 / 3628800;
-    e = __builtin_fma(e, r, 1.0 / 362880);
-    e = __builtin_fma(e, r, 1.0 / 40320);
-    e = __builtin_fma(e, r, 1.0 / 5040);
-    e = __builtin_fma(e, r, 1.0 / 720);
-    e = __builtin_fma(e, r, 1.0 / 120);
-    e = __builtin_fma(e, r, 1.0 / 24);
-    e = __builtin_fma(e, r, 1.0 / 6);
-    e = __builtin_fma(e, r, 0.5);
-    e = __builtin_fma(e, r, 1.0);
-    e = __builtin_fma(e, r, 1.0);
-    const double scaled = __hiloint2double(__double2hiint(e) + (__double2loint(t) << 20), __double2loint(e));  // e 2^k
-    return y >= -700.0 ? scaled : 0.0;
-}
-
-// weight of a logit against the largest one, m: exp((x - m) / T); 0 for -inf and
-// for what is not a number, 1 for m itself (also where it is +inf)
-__device__ inline double weight(float x, float m, double inv_t) {
-    const double y = __builtin_fmax(((double)x - (double)m) * inv_t, kNothing);  // (NaN: kNothing)
-    return x == m ? 1.0 : exp_neg(y);
-}
+// Weights exp((x - m) / T) = 2^z, z = (x - m) log2(e) / T, in f64.  z = k + f
+// with k by adding and taking away 1.5 2^52 (which leaves it in the sum's low
+// bits), |f| <= 1/2, and 2^f by its Taylor series to f^10 (the next term is below
+// 2.3e-13); the factor and the product round by 2^-53 of |z|, below 100 or so.
+struct Weigher {
+    double c, top;
+    bool inf;  // the largest logit is +inf: it weighs 1, all others 0
+    __device__ Weigher(float m, float t) : c(1.4426950408889634074 / (double)t), top(m), inf(m == INFINITY) {}
+    // 0 for -inf and for what is not a number (z at least -2000: scaled to 0)
+    __device__ __forceinline__ double operator()(float x) const {
+        constexpr double kRound = 6755399441055744.0, l = 0.69314718055994530942;
+        constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6,
+                         c7 = c6 * l / 7, c8 = c7 * l / 8, c9 = c8 * l / 9, c10 = c9 * l / 10;
+        const double z = __builtin_fmax(((double)x - top) * c, -2000.0);  // (NaN: -2000)
+        const double t = z + kRound, f = z - (t - kRound);
+        double e = __builtin_fma(c10, f, c9);
+        e = __builtin_fma(e, f, c8);
+        e = __builtin_fma(e, f, c7);
+        e = __builtin_fma(e, f, c6);
+        e = __builtin_fma(e, f, c5);
+        e = __builtin_fma(e, f, c4);
+        e = __builtin_fma(e, f, c3);
+        e = __builtin_fma(e, f, c2);
+        e = __builtin_fma(e, f, l);
+        e = __builtin_fma(e, f, 1.0);
+        return __builtin_ldexp(e, __double2loint(t));
+    }
+};
 // the same in f32: c = log2(e) / T
 __device__ inline float weight32(float x, float m, float c) {
     const float y = fmaxf((x - m) * c, -1000.0f);  // (NaN: nothing)
     return x == m ? 1.0f : __builtin_amdgcn_exp2f(y);
 }
 
-__device__ inline double shfl_xor64(double v, int mask) {
-    return __hiloint2double(__shfl_xor(__double2hiint(v), mask, 64), __shfl_xor(__double2loint(v), mask, 64));
+// Lanes meet over DPP (rows of 16 lanes, every lane active in a row that takes
+// part) and, between rows, over readlane: a step costs tens of cycles less than a
+// shuffle through LDS, and these kernels are chains of such steps.
+constexpr int kRowRor = 0x120, kRowShr = 0x110;  // + lanes; shr fills with 0
+template <int CTRL> __device__ inline int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
+template <int CTRL> __device__ inline float dpp(float v) { return __int_as_float(dpp<CTRL>(__float_as_int(v))); }
+template <int CTRL> __device__ inline double dpp(double v) {
+    return __hiloint2double(dpp<CTRL>(__double2hiint(v)), dpp<CTRL>(__double2loint(v)));
 }
-__device__ inline double shfl_up64(double v, int by) {
-    return __hiloint2double(__shfl_up(__double2hiint(v), by, 64), __shfl_up(__double2loint(v), by, 64));
+__device__ inline int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ inline float lane_of(float v, int lane) { return __int_as_float(lane_of(__float_as_int(v), lane)); }
+__device__ inline double lane_of(double v, int lane) {
+    return __hiloint2double(lane_of(__double2hiint(v), lane), lane_of(__double2loint(v), lane));
+}
+// sums: of a row of 16 lanes, of the wave (the same bits in every lane)
+template <typename T> __device__ inline T row_sum(T v) {
+    v += dpp<kRowRor + 8>(v);
+    v += dpp<kRowRor + 4>(v);
+    v += dpp<kRowRor + 2>(v);
+    v += dpp<kRowRor + 1>(v);
+    return v;
+}
+template <typename T> __device__ inline T wave_sum(T v) {
+    v = row_sum(v);
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+// the sum of the lanes up to and with this one
+__device__ inline double wave_scan(double v, int lane) {
+    v += dpp<kRowShr + 1>(v);
+    v += dpp<kRowShr + 2>(v);
+    v += dpp<kRowShr + 4>(v);
+    v += dpp<kRowShr + 8>(v);
+    const double r0 = lane_of(v, 15), r1 = r0 + lane_of(v, 31), r2 = r1 + lane_of(v, 47);
+    return v + (lane < 16 ? 0.0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
 }
 // the larger logit, the lower column among equals
 __device__ inline void take_larger(float& m, int& at, float m2, int at2) {
@@ -133,9 +162,20 @@ __device__ inline void take_larger(float& m, int& at, float m2, int at2) {
         at = at2;
     }
 }
+__device__ inline void row_larger(float& m, int& at) {
+    take_larger(m, at, dpp<kRowRor + 8>(m), dpp<kRowRor + 8>(at));
+    take_larger(m, at, dpp<kRowRor + 4>(m), dpp<kRowRor + 4>(at));
+    take_larger(m, at, dpp<kRowRor + 2>(m), dpp<kRowRor + 2>(at));
+    take_larger(m, at, dpp<kRowRor + 1>(m), dpp<kRowRor + 1>(at));
+}
 __device__ inline void wave_larger(float& m, int& at) {
+    row_larger(m, at);
+    float top = lane_of(m, 0);
+    int col = lane_of(at, 0);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) take_larger(m, at, __shfl_xor(m, off, 64), __shfl_xor(at, off, 64));
+    for (int r = 16; r < 64; r += 16) take_larger(top, col, lane_of(m, r), lane_of(at, r));
+    m = top;
+    at = col;
 }
 
 __device__ inline int seq_of(const VerifyArgs& v, int n, int row) {
@@ -155,7 +195,6 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyA
     __shared__ int sat[4];
     __shared__ float ss[4];
     const int row = blockIdx.x / b.chunks, ch = blockIdx.x - row * b.chunks;
-    const float t = v.temp[seq_of(v, n, row)];
     const int c0 = ch * b.chunk, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* x = b.logits + (size_t)row * b.cols;
     float4 d[E];
@@ -173,6 +212,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyA
             d[e].w = c1 + 768 < b.cols ? x[c1 + 768] : none;
         }
     }
+    const float t = v.temp[seq_of(v, n, row)];  // (behind the loads' issue: a chain of scalar loads)
     float m = -INFINITY;
     int at = c0;
 #pragma unroll
@@ -199,9 +239,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyA
             sum += weight32(d[e].z, m, c);
             s2 += weight32(d[e].w, m, c);
         }
-        sum += s2;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        sum = wave_sum(sum + s2);
     }
     if (lane == 0) {
         sm[wave] = m;
@@ -245,8 +283,7 @@ __device__ inline Decision decide(const VerifyBufs& b, const VerifyArgs& v, int 
                 at = x.at;
             }
         }
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) take_larger(m, at, __shfl_xor(m, off, 64), __shfl_xor(at, off, 64));
+        row_larger(m, at);
         if (m == -INFINITY) at = 0;  // a row without a finite logit: the first place, as the argmax has it
         float z = 0.0f;
         if (t > 0.0f && m != -INFINITY)
@@ -254,126 +291,129 @@ __device__ inline Decision decide(const VerifyBufs& b, const VerifyArgs& v, int 
                 const ChunkStat x = st[c];
                 if (x.m != -INFINITY) z += x.sum * weight32(x.m, m, c32);
             }
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) z += __shfl_xor(z, off, 64);
+        z = row_sum(z);
         if (lane == 0) {
             sm[i] = m;
             sat[i] = at;
             sz[i] = z;
             ok[i] = t <= 0.0f ? y == (uint32_t)at
-                              : m != -INFINITY && (double)u * (double)qy * (double)z < weight(xy, m, 1.0 / (double)t);
+                              : m != -INFINITY && (double)u * (double)qy * (double)z < (m == INFINITY ? (xy == m ? 1.0 : 0.0) : Weigher(m, t)(xy));
         }
     }
     __syncthreads();
     int a = 0;
-    while (a < k && ok[a]) ++a;
-    return {k, a, row0 + a, sm[a], sat[a], sz[a], t, 0};
-}
-
-// Where the emission row's weights come from: of p, or of the rest that the
-// rejected draft leaves.
-struct Rest {
-    const float* x;
-    const float* q;  // the rejected draft's probabilities, or null: p ...
-    uint32_t out;    // ... without a certain draft's own column (none: 0xffffffff)
-};
-__device__ inline Rest rest_of(const VerifyBufs& b, const VerifyArgs& v, int s, const Decision& d) {
-    const size_t at = (size_t)(v.row[s] - s + d.accepted);
-    const bool left = d.accepted < d.drafts;
-    return {b.logits + (size_t)d.row * b.cols, left && b.probs ? b.probs + at * b.cols : nullptr,
-            left && !b.probs ? b.drafts[at] : 0xffffffffu};
-}
-
-__device__ inline double wave_sum(double v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += shfl_xor64(v, off);
-    return v;
-}
-
-template <bool VEC>
-__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyArgs v) {
-    __shared__ double ss[3][4];
-    constexpr int E = kRestChunk / 256;
-    const int s = blockIdx.x / b.rest_chunks, ch = blockIdx.x - s * b.rest_chunks, tid = threadIdx.x;
-    const Decision d = decide(b, v, s);
-    if (ch == 0 && tid == 0) b.dec[s] = d;
-    if (d.t <= 0.0f || d.z <= 0.0f) return;  // greedy, or nothing weighs: the first largest logit
-    const Rest r = rest_of(b, v, s, d);
-    const int c0 = ch * kRestChunk;
-    float x[E], q[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        x[e] = -INFINITY;
-        q[e] = 0.0f;
-    }
-    if constexpr (VEC) {
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-            const int c = c0 + e * 256 + tid * 4;
-            if (c < b.cols) {
-                *(float4*)(x + e) = *(const float4*)(r.x + c);
-                if (r.q) *(float4*)(q + e) = *(const float4*)(r.q + c);
-            }
+    for (;;) {  // (64 drafts at a time: the first rejected one)
+        const int i = a + (tid & 63);
+        const unsigned long long no = __ballot(i >= k || !ok[i]);
+        if (no) {
+            a += __ffsll(no) - 1;
+            break;
         }
-    } else {
+        a += 64;
+    }
+    const bool left = a < k;  // a draft was rejected
+    return {sm[a], sat[a], sz[a], t, row0 + a, left && b.probs ? d0 + a : -1, left && !b.probs ? b.drafts[d0 + a] : 0xffffffffu,
+            b.u[row0 + k], k, a};
+}
+
+// A workgroup takes `per` chunks of one sequence's emission row in turn: as many as
+// leave no more workgroups than the chip holds at once, for each has the tests to do first.
+template <bool VEC>
+__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyArgs v, int per, int groups) {
+    __shared__ double ss[2][3][4];
+    constexpr int E = kRestChunk / 256;
+    const int s = blockIdx.x / groups, g = blockIdx.x - s * groups, tid = threadIdx.x;
+    const Decision d = decide(b, v, s);
+    if (g == 0 && tid == 0) b.dec[s] = d;
+    if (d.t <= 0.0f || d.z <= 0.0f) return;  // greedy, or nothing weighs: the first largest logit
+    const float* xr = b.logits + (size_t)d.row * b.cols;
+    const float* qr = d.probs >= 0 ? b.probs + (size_t)d.probs * b.cols : nullptr;
+    const Weigher weight(d.m, d.t);
+    const int end = min((g + 1) * per, b.rest_chunks);
+    for (int ch = g * per; ch < end; ++ch) {
+        const int c0 = ch * kRestChunk, buf = ch & 1;
+        float x[E], q[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int c = c0 + e * 256 + tid;
-            if (c < b.cols) {
-                x[e] = r.x[c];
-                if (r.q) q[e] = r.q[c];
+            x[e] = -INFINITY;
+            q[e] = 0.0f;
+        }
+        if constexpr (VEC) {
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                const int c = c0 + e * 256 + tid * 4;
+                if (c < b.cols) {
+                    *(float4*)(x + e) = *(const float4*)(xr + c);
+                    if (qr) *(float4*)(q + e) = *(const float4*)(qr + c);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int c = c0 + e * 256 + tid;
+                if (c < b.cols) {
+                    x[e] = xr[c];
+                    if (qr) q[e] = qr[c];
+                }
             }
         }
-    }
-    const double inv_t = 1.0 / (double)d.t, z = d.z;
-    double w = 0.0, wa = 0.0, qa = 0.0;
+        double w = 0.0, wa = 0.0, qa = 0.0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = VEC ? c0 + (e / 4) * 1024 + tid * 4 + (e & 3) : c0 + e * 256 + tid;
-        const double we = weight(x[e], d.m, inv_t), qe = fmaxf(q[e], 0.0f);
-        w += we;
-        const bool in = r.q ? we > qe * z : (uint32_t)c != r.out;
-        wa += in ? we : 0.0;
-        qa += in ? qe : 0.0;
-    }
-    w = wave_sum(w);
-    wa = wave_sum(wa);
-    qa = wave_sum(qa);
-    if ((tid & 63) == 0) {
-        ss[0][tid >> 6] = w;
-        ss[1][tid >> 6] = wa;
-        ss[2][tid >> 6] = qa;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        double o[3];
+        for (int e = 0; e < E; ++e) {
+            const int c = VEC ? c0 + (e / 4) * 1024 + tid * 4 + (e & 3) : c0 + e * 256 + tid;
+            const double we = weight.inf ? (x[e] == d.m ? 1.0 : 0.0) : weight(x[e]);
+            const float qe = fmaxf(q[e], 0.0f);
+            w += we;
+            const bool in = qr ? (float)we > qe * d.z : (uint32_t)c != d.out;
+            wa += in ? we : 0.0;
+            qa += (double)(in ? qe : 0.0f);
+        }
+        w = wave_sum(w);
+        wa = wave_sum(wa);
+        qa = wave_sum(qa);
+        if ((tid & 63) == 0) {
+            ss[buf][0][tid >> 6] = w;
+            ss[buf][1][tid >> 6] = wa;
+            ss[buf][2][tid >> 6] = qa;
+        }
+        __syncthreads();  // (one a chunk: two buffers, in turn)
+        if (tid == 0) {
+            double o[3];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) o[i] = (ss[i][0] + ss[i][1]) + (ss[i][2] + ss[i][3]);
-        b.rest[(size_t)s * b.rest_chunks + ch] = {o[0], o[1], o[2]};
+            for (int i = 0; i < 3; ++i) o[i] = (ss[buf][i][0] + ss[buf][i][1]) + (ss[buf][i][2] + ss[buf][i][3]);
+            b.rest[(size_t)s * b.rest_chunks + ch] = {o[0], o[1], o[2]};
+        }
     }
 }
 
-// A workgroup of 4 waves per sequence.
-__global__ __launch_bounds__(256) void verify_emit_kernel(VerifyBufs b, VerifyArgs v) {
-    __shared__ double sw[4];
+// A workgroup of 16 waves per sequence.  A chain of latencies: what can be loaded
+// before the decision is known is, and two columns a thread keep the code short
+// (its first pass waits for every line of it).
+constexpr int kEmitThreads = 1024;
+__global__ __launch_bounds__(kEmitThreads) void verify_emit_kernel(VerifyBufs b, VerifyArgs v) {
+    __shared__ double sw[kEmitThreads / 64];
     __shared__ double s_before, s_target, s_z;
     __shared__ int s_chunk, s_first, s_last;
     __shared__ bool s_whole;
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const RestSum* rs = b.rest + (size_t)s * b.rest_chunks;
+    const RestSum mine = rs[min(lane, b.rest_chunks - 1)];  // the lane's first chunk (of a greedy row: not used)
+    const uint32_t y = tid < v.row[s + 1] - v.row[s] - 1 ? b.drafts[v.row[s] - s + tid] : 0;  // (at most 255 drafts)
     const Decision d = b.dec[s];
     uint32_t token = (uint32_t)d.at;
     if (d.t > 0.0f && d.z > 0.0f) {
-        const Rest r = rest_of(b, v, s, d);
+        const float* xr = b.logits + (size_t)d.row * b.cols;
+        const float* qr = d.probs >= 0 ? b.probs + (size_t)d.probs * b.cols : nullptr;
+        const Weigher weight(d.m, d.t);
         if (wave == 0) {
-            const RestSum* rs = b.rest + (size_t)s * b.rest_chunks;
-            const double u = b.u[v.row[s] + d.drafts];
+            auto sum_of = [&](int c) { return c < 64 ? mine : rs[c]; };
             double z = 0.0, total = 0.0;
-            for (int c = lane; c < b.rest_chunks; c += 64) z += rs[c].w;
+            for (int c = lane; c < b.rest_chunks; c += 64) z += sum_of(c).w;
             z = wave_sum(z);
             bool whole = false;  // the rest weighs nothing (by rounding): the token comes from p
             auto chunk_sum = [&](int c) {
-                const RestSum x = rs[c];
-                return whole ? x.w : r.q ? __builtin_fmax(__builtin_fma(-x.qa, z, x.wa), 0.0) : x.wa;
+                const RestSum x = sum_of(c);
+                return whole ? x.w : qr ? __builtin_fmax(__builtin_fma(-x.qa, z, x.wa), 0.0) : x.wa;
             };
             for (int pass = 0; pass < 2; ++pass) {
                 total = 0.0;
@@ -382,29 +422,22 @@ __global__ __launch_bounds__(256) void verify_emit_kernel(VerifyBufs b, VerifyAr
                 if (total > 0.0) break;
                 whole = true;
             }
-            const double target = u * total;
+            const double target = (double)d.u * total;
             // the first chunk whose end exceeds the target; none (u >= 1 or not a number): the last that weighs
             double before = 0.0, pick_before = 0.0;
             int chunk = 0;
             bool found = false;
             for (int c0 = 0; c0 < b.rest_chunks && !found; c0 += 64) {
                 const double w = c0 + lane < b.rest_chunks ? chunk_sum(c0 + lane) : 0.0;
-                double run = w;
-#pragma unroll
-                for (int off = 1; off < 64; off <<= 1) {
-                    const double up = shfl_up64(run, off);
-                    if (lane >= off) run += up;
-                }
+                const double run = wave_scan(w, lane);
                 const unsigned long long hit = __ballot(w > 0.0 && before + run > target), some = __ballot(w > 0.0);
-                const double up1 = shfl_up64(run, 1), start = lane ? up1 : 0.0;  // (every lane takes part in the shuffle)
                 if (some) {
                     const int pick = hit ? __ffsll(hit) - 1 : 63 - __clzll(some);
                     chunk = c0 + pick;
-                    pick_before = before + __hiloint2double(__shfl(__double2hiint(start), pick, 64),
-                                                            __shfl(__double2loint(start), pick, 64));
+                    pick_before = before + (pick ? lane_of(run, pick - 1) : 0.0);
                     found = hit != 0;
                 }
-                before += __hiloint2double(__shfl(__double2hiint(run), 63, 64), __shfl(__double2loint(run), 63, 64));
+                before += lane_of(run, 63);
             }
             if (lane == 0) {
                 s_chunk = chunk;
@@ -418,29 +451,24 @@ __global__ __launch_bounds__(256) void verify_emit_kernel(VerifyBufs b, VerifyAr
         }
         __syncthreads();
         // the chunk's columns, E to a thread, in order
-        constexpr int E = kRestChunk / 256;
+        constexpr int E = kRestChunk / kEmitThreads;
         const int c0 = s_chunk * kRestChunk + tid * E;
-        const double inv_t = 1.0 / (double)d.t, z = s_z;
+        const double z = s_z;
         const bool whole = s_whole;
         float x[E], q[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            x[e] = c0 + e < b.cols ? r.x[c0 + e] : -INFINITY;
-            q[e] = r.q && c0 + e < b.cols ? fmaxf(r.q[c0 + e], 0.0f) : 0.0f;
+            x[e] = c0 + e < b.cols ? xr[c0 + e] : -INFINITY;
+            q[e] = qr && c0 + e < b.cols ? fmaxf(qr[c0 + e], 0.0f) : 0.0f;
         }
         double w[E], sum = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            w[e] = weight(x[e], d.m, inv_t);
-            if (!whole) w[e] = r.q ? __builtin_fmax(w[e] - (double)q[e] * z, 0.0) : (uint32_t)(c0 + e) == r.out ? 0.0 : w[e];
+            w[e] = weight.inf ? (x[e] == d.m ? 1.0 : 0.0) : weight(x[e]);
+            if (!whole) w[e] = qr ? __builtin_fmax(w[e] - (double)q[e] * z, 0.0) : (uint32_t)(c0 + e) == d.out ? 0.0 : w[e];
             sum += w[e];
         }
-        double run = sum;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const double up = shfl_up64(run, off);
-            if (lane >= off) run += up;
-        }
+        const double run = wave_scan(sum, lane);
         if (lane == 63) sw[wave] = run;
         __syncthreads();
         double cum = s_before;
@@ -461,9 +489,8 @@ __global__ __launch_bounds__(256) void verify_emit_kernel(VerifyBufs b, VerifyAr
         // (no crossing: the chunk's sum and this one's order differ in their last bits, or u >= 1)
         token = s_first != 0x7fffffff ? (uint32_t)s_first : s_last >= 0 ? (uint32_t)s_last : (uint32_t)d.at;
     }
-    const uint32_t* y = b.drafts + (v.row[s] - s);
-    for (int i = tid; i < b.out_stride; i += 256)
-        b.out[(size_t)s * b.out_stride + i] = i < d.accepted ? y[i] : i == d.accepted ? token : 0xffffffffu;
+    for (int i = tid; i < b.out_stride; i += kEmitThreads)
+        b.out[(size_t)s * b.out_stride + i] = i < d.accepted ? y : i == d.accepted ? token : 0xffffffffu;
     if (tid == 0) b.accepted[s] = d.accepted;
 }
 
@@ -533,12 +560,13 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
             default: if (vec) stats(verify_stats_kernel<8, true>); else stats(verify_stats_kernel<8, false>); break;
         }
         ZR_LAUNCH_CHECK(ctx);
+        const int per = (m * rest_chunks + 2047) / 2048, groups = (rest_chunks + per - 1) / per;
         if (vec && ((uintptr_t)vb->d_draft_probs & 15) == 0)
-            hipLaunchKernelGGL(verify_rest_kernel<true>, dim3(m * rest_chunks), dim3(256), 0, ctx->stream, b, v);
+            hipLaunchKernelGGL(verify_rest_kernel<true>, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
         else
-            hipLaunchKernelGGL(verify_rest_kernel<false>, dim3(m * rest_chunks), dim3(256), 0, ctx->stream, b, v);
+            hipLaunchKernelGGL(verify_rest_kernel<false>, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
         ZR_LAUNCH_CHECK(ctx);
-        hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(256), 0, ctx->stream, b, v);
+        hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(kEmitThreads), 0, ctx->stream, b, v);
         ZR_LAUNCH_CHECK(ctx);
         row0 += r;
         draft0 += r - m;
