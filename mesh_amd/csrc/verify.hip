@@ -483,8 +483,10 @@ __global__ __launch_bounds__(kEmitThreads) void verify_emit_kernel(VerifyBufs b,
                 if (first == 0x7fffffff && cum > s_target) first = c0 + e;
             }
         }
-        if (first != 0x7fffffff) atomicMin(&s_first, first);
-        if (last >= 0) atomicMax(&s_last, last);
+        // (a wave's columns ascend with its lanes; one atomic a wave: every lane's own took 5 us)
+        const unsigned long long hit = __ballot(first != 0x7fffffff), some = __ballot(last >= 0);
+        if (hit && lane == __ffsll(hit) - 1) atomicMin(&s_first, first);
+        if (some && lane == 63 - __clzll(some)) atomicMax(&s_last, last);
         __syncthreads();
         // (no crossing: the chunk's sum and this one's order differ in their last bits, or u >= 1)
         token = s_first != 0x7fffffff ? (uint32_t)s_first : s_last >= 0 ? (uint32_t)s_last : (uint32_t)d.at;
