@@ -11,10 +11,11 @@
 namespace zr {
 
 // Pairs travel as a kernel argument (at most 4 KiB of them): nothing is staged,
-// so the call returns with its arrays free and later calls share no buffer.
-constexpr int kPairsPerLaunch = 448;
-struct PagePairs {
-    int src[kPairsPerLaunch], dst[kPairsPerLaunch];
+// so the call returns with its arrays free and later calls share no buffer.  A
+// few (a fork's first writes) go as a small one, which costs the host less.
+constexpr int kPairsPerLaunch = 448, kFewPairs = 32;
+template <int N> struct PagePairs {
+    int src[N], dst[N];
 };
 
 // A workgroup copies 16 KiB of one pair's page in one layer: 4 loads of 16 B
@@ -22,8 +23,9 @@ struct PagePairs {
 constexpr int kCopyVecs = 4;
 constexpr int kCopyChunk = 256 * kCopyVecs * 16;  // bytes
 
+template <int N>
 __global__ __launch_bounds__(256) void kv_copy_pages_kernel(unsigned char* pool, size_t layer_bytes, uint32_t page_bytes,
-                                                            int chunks, PagePairs pp) {
+                                                            int chunks, PagePairs<N> pp) {
     const int pair = blockIdx.x / chunks, chunk = blockIdx.x - pair * chunks;
     unsigned char* layer = pool + (size_t)blockIdx.y * layer_bytes;
     const uint4* src = (const uint4*)(layer + (size_t)pp.src[pair] * page_bytes);
@@ -38,23 +40,25 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(unsigned char* pool,
         if (v0 + 256 * i < vecs) dst[v0 + 256 * i] = x[i];
 }
 
-zr_status launch_kv_copy_pages(zr_context* ctx, const int* src, const int* dst, int n) {
-    if (n <= 0) return ZR_OK;
+template <int N> static void launch_pairs(zr_context* ctx, const int* src, const int* dst, int m) {
     // a page is 2 kv_cols x 16 elements, kv_cols a multiple of 4: whole 16-byte vectors
     const int chunks = (int)((ctx->page_bytes + kCopyChunk - 1) / kCopyChunk);
+    PagePairs<N> pp;
+    for (int j = 0; j < N; ++j) {  // (past m: never read)
+        pp.src[j] = j < m ? src[j] : 0;
+        pp.dst[j] = j < m ? dst[j] : 0;
+    }
+    hipLaunchKernelGGL(kv_copy_pages_kernel<N>, dim3(m * chunks, ctx->desc.num_layers), dim3(256), 0, ctx->stream,
+                       (unsigned char*)ctx->kv_pool, ctx->page_bytes * ctx->n_pages, (uint32_t)ctx->page_bytes, chunks, pp);
+}
+
+zr_status launch_kv_copy_pages(zr_context* ctx, const int* src, const int* dst, int n) {
+    if (n <= 0) return ZR_OK;
     hipEvent_t ev;
     timing_mark_begin(ctx, kClassOther, &ev);
     for (int i = 0; i < n; i += kPairsPerLaunch) {
         const int m = std::min(kPairsPerLaunch, n - i);
-        PagePairs pp;
-        for (int j = 0; j < m; ++j) {
-            pp.src[j] = src[i + j];
-            pp.dst[j] = dst[i + j];
-        }
-        for (int j = m; j < kPairsPerLaunch; ++j) pp.src[j] = pp.dst[j] = 0;  // never read
-        hipLaunchKernelGGL(kv_copy_pages_kernel, dim3(m * chunks, ctx->desc.num_layers), dim3(256), 0, ctx->stream,
-                           (unsigned char*)ctx->kv_pool, ctx->page_bytes * ctx->n_pages, (uint32_t)ctx->page_bytes,
-                           chunks, pp);
+        if (m <= kFewPairs) launch_pairs<kFewPairs>(ctx, src + i, dst + i, m); else launch_pairs<kPairsPerLaunch>(ctx, src + i, dst + i, m);
         ZR_LAUNCH_CHECK(ctx);
     }
     timing_mark_end(ctx, kClassOther, ev);

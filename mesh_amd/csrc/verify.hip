@@ -42,9 +42,12 @@ constexpr int kMaxDrafts = 255;   // drafts of one sequence
 constexpr int kRestChunk = 2048;  // columns of an emission row's chunk
 constexpr float kLog2E = 1.44269504088896341f;
 
-struct VerifyArgs {
-    int row[kSeqs + 1];    // first logits row of each sequence, and the end; drafts before it: row[s] - s
-    float temp[kSeqs];
+// Sequences of a launch, as a kernel argument: N = 16 or kSeqs (2 KiB of arguments
+// cost the host half a microsecond a launch: 5 rows of 32000 15.5 us with them, 13.7 without).
+constexpr int kFewSeqs = 16;
+template <int N> struct VerifyArgs {
+    int row[N + 1];    // first logits row of each sequence, and the end; drafts before it: row[s] - s
+    float temp[N];
 };
 
 struct VerifyBufs {
@@ -83,7 +86,7 @@ struct Decision {
     int probs;     // ... of the rejected draft's probabilities, or -1: p ...
     uint32_t out;  // ... without a certain draft's own column (none: 0xffffffff)
     float u;
-    int drafts, accepted;
+    int first, accepted;  // the sequence's first draft; how many were accepted
 };
 
 // Weights exp((x - m) / T) = 2^z, z = (x - m) log2(e) / T, in f64.  z = k + f
@@ -178,7 +181,7 @@ __device__ inline void wave_larger(float& m, int& at) {
     at = col;
 }
 
-__device__ inline int seq_of(const VerifyArgs& v, int n, int row) {
+template <int N> __device__ inline int seq_of(const VerifyArgs<N>& v, int n, int row) {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -189,8 +192,8 @@ __device__ inline int seq_of(const VerifyArgs& v, int n, int row) {
 
 // A workgroup of 4 waves takes one chunk of 1024 E columns of one row; every
 // load of a lane goes out before the first is used.
-template <int E, bool VEC>
-__global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyArgs v, int n) {
+template <int E, bool VEC, int N>
+__global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyArgs<N> v, int n) {
     __shared__ float sm[4];
     __shared__ int sat[4];
     __shared__ float ss[4];
@@ -261,7 +264,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyA
 // The tests of a sequence, by 16 groups of 16 lanes, a row each in turn: the
 // chunks' sums joined in one order, so every workgroup gets the same bits.  The
 // draft's own logit and probability come beside them.
-__device__ inline Decision decide(const VerifyBufs& b, const VerifyArgs& v, int s) {
+template <int N> __device__ inline Decision decide(const VerifyBufs& b, const VerifyArgs<N>& v, int s) {
     __shared__ float sm[kMaxDrafts + 1], sz[kMaxDrafts + 1];
     __shared__ int sat[kMaxDrafts + 1], ok[kMaxDrafts + 1];
     const int tid = threadIdx.x, lane = tid & 15;
@@ -313,13 +316,13 @@ __device__ inline Decision decide(const VerifyBufs& b, const VerifyArgs& v, int 
     }
     const bool left = a < k;  // a draft was rejected
     return {sm[a], sat[a], sz[a], t, row0 + a, left && b.probs ? d0 + a : -1, left && !b.probs ? b.drafts[d0 + a] : 0xffffffffu,
-            b.u[row0 + k], k, a};
+            b.u[row0 + k], d0, a};
 }
 
 // A workgroup takes `per` chunks of one sequence's emission row in turn: as many as
 // leave no more workgroups than the chip holds at once, for each has the tests to do first.
-template <bool VEC>
-__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyArgs v, int per, int groups) {
+template <bool VEC, int N>
+__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyArgs<N> v, int per, int groups) {
     __shared__ double ss[2][3][4];
     constexpr int E = kRestChunk / 256;
     const int s = blockIdx.x / groups, g = blockIdx.x - s * groups, tid = threadIdx.x;
@@ -390,7 +393,7 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyAr
 // before the decision is known is, and two columns a thread keep the code short
 // (its first pass waits for every line of it).
 constexpr int kEmitThreads = 1024;
-__global__ __launch_bounds__(kEmitThreads) void verify_emit_kernel(VerifyBufs b, VerifyArgs v) {
+__global__ __launch_bounds__(kEmitThreads) void verify_emit_kernel(VerifyBufs b) {
     __shared__ double sw[kEmitThreads / 64];
     __shared__ double s_before, s_target, s_z;
     __shared__ int s_chunk, s_first, s_last;
@@ -398,8 +401,8 @@ __global__ __launch_bounds__(kEmitThreads) void verify_emit_kernel(VerifyBufs b,
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const RestSum* rs = b.rest + (size_t)s * b.rest_chunks;
     const RestSum mine = rs[min(lane, b.rest_chunks - 1)];  // the lane's first chunk (of a greedy row: not used)
-    const uint32_t y = tid < v.row[s + 1] - v.row[s] - 1 ? b.drafts[v.row[s] - s + tid] : 0;  // (at most 255 drafts)
     const Decision d = b.dec[s];
+    const uint32_t y = tid < d.accepted ? b.drafts[d.first + tid] : 0;  // (at most 255 drafts)
     uint32_t token = (uint32_t)d.at;
     if (d.t > 0.0f && d.z > 0.0f) {
         const float* xr = b.logits + (size_t)d.row * b.cols;
@@ -496,6 +499,34 @@ __global__ __launch_bounds__(kEmitThreads) void verify_emit_kernel(VerifyBufs b,
     if (tid == 0) b.accepted[s] = d.accepted;
 }
 
+// The pass over all logits and that over the emission rows of m <= N sequences.
+template <int N>
+void launch_passes(zr_context* ctx, const VerifyBufs& b, const int* draft_len, const float* temperature, int m, int e,
+                   bool vec, bool rest_vec) {
+    VerifyArgs<N> v;
+    int r = 0;
+    for (int s = 0; s < N; ++s) {
+        v.row[s] = r;
+        v.temp[s] = s < m ? temperature[s] : 0.0f;
+        if (s < m) r += draft_len[s] + 1;
+    }
+    v.row[N] = r;
+    auto stats = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(r * b.chunks), dim3(256), 0, ctx->stream, b, v, m);
+    };
+    switch (e) {
+        case 1: if (vec) stats(verify_stats_kernel<1, true, N>); else stats(verify_stats_kernel<1, false, N>); break;
+        case 2: if (vec) stats(verify_stats_kernel<2, true, N>); else stats(verify_stats_kernel<2, false, N>); break;
+        case 4: if (vec) stats(verify_stats_kernel<4, true, N>); else stats(verify_stats_kernel<4, false, N>); break;
+        default: if (vec) stats(verify_stats_kernel<8, true, N>); else stats(verify_stats_kernel<8, false, N>); break;
+    }
+    const int per = (m * b.rest_chunks + 2047) / 2048, groups = (b.rest_chunks + per - 1) / per;
+    auto rest = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
+    };
+    if (rest_vec) rest(verify_rest_kernel<true, N>); else rest(verify_rest_kernel<false, N>);
+}
+
 }  // namespace
 
 zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const zr_verify_batch* vb, uint32_t* d_out,
@@ -528,14 +559,8 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
     size_t row0 = 0, draft0 = 0;
     for (int s0 = 0; s0 < n; s0 += kSeqs) {
         const int m = std::min(kSeqs, n - s0);
-        VerifyArgs v;
         int r = 0;
-        for (int s = 0; s < kSeqs; ++s) {
-            v.row[s] = r;
-            v.temp[s] = s < m ? vb->temperature[s0 + s] : 0.0f;
-            if (s < m) r += vb->draft_len[s0 + s] + 1;
-        }
-        v.row[kSeqs] = r;
+        for (int s = 0; s < m; ++s) r += vb->draft_len[s0 + s] + 1;
         VerifyBufs b;
         b.logits = d_logits + row0 * cols;
         b.cols = cols;
@@ -552,23 +577,15 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
         b.out_stride = out_stride;
         b.accepted = d_accepted + s0;
         const bool vec = cols % 4 == 0 && ((uintptr_t)d_logits & 15) == 0;
-        auto stats = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(r * chunks), dim3(256), 0, ctx->stream, b, v, m);
-        };
-        switch (e) {
-            case 1: if (vec) stats(verify_stats_kernel<1, true>); else stats(verify_stats_kernel<1, false>); break;
-            case 2: if (vec) stats(verify_stats_kernel<2, true>); else stats(verify_stats_kernel<2, false>); break;
-            case 4: if (vec) stats(verify_stats_kernel<4, true>); else stats(verify_stats_kernel<4, false>); break;
-            default: if (vec) stats(verify_stats_kernel<8, true>); else stats(verify_stats_kernel<8, false>); break;
-        }
-        ZR_LAUNCH_CHECK(ctx);
-        const int per = (m * rest_chunks + 2047) / 2048, groups = (rest_chunks + per - 1) / per;
-        if (vec && ((uintptr_t)vb->d_draft_probs & 15) == 0)
-            hipLaunchKernelGGL(verify_rest_kernel<true>, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
+        const int *lens = vb->draft_len + s0;
+        const float* temps = vb->temperature + s0;
+        const bool rest_vec = vec && ((uintptr_t)vb->d_draft_probs & 15) == 0;
+        if (m <= kFewSeqs)
+            launch_passes<kFewSeqs>(ctx, b, lens, temps, m, e, vec, rest_vec);
         else
-            hipLaunchKernelGGL(verify_rest_kernel<false>, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
+            launch_passes<kSeqs>(ctx, b, lens, temps, m, e, vec, rest_vec);
         ZR_LAUNCH_CHECK(ctx);
-        hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(kEmitThreads), 0, ctx->stream, b, v);
+        hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(kEmitThreads), 0, ctx->stream, b);
         ZR_LAUNCH_CHECK(ctx);
         row0 += r;
         draft0 += r - m;
