@@ -2244,16 +2244,26 @@ zr_status zr_forward_verify(zr_context* ctx, const zr_microbatch* mb, const floa
         return set_err(ctx, ZR_E_INVALID, "null argument");
     ZR_HIP(ctx, hipSetDevice(ctx->device));
     const int n = mb->num_seqs, V = ctx->desc.vocab;
-    StagedMeta* st = ctx->scratch_stage;
-    if (zr_status rc = stage_microbatch(ctx, mb, st)) return rc;  // (checks the counts, the rows and the token ids)
-    const int T = st->total_q;
+    if (n <= 0 || n > ctx->desc.max_seqs)
+        return set_err(ctx, ZR_E_INVALID, "verification of %d sequences (capacity %d)", n, ctx->desc.max_seqs);
+    std::vector<int> lens(n);
+    long rows = 0;
+    for (int s = 0; s < n; ++s) {
+        if (mb->q_len[s] <= 0) return set_err(ctx, ZR_E_INVALID, "sequence %d has q_len %d", s, mb->q_len[s]);
+        lens[s] = mb->q_len[s] - 1;
+        rows += mb->q_len[s];
+    }
+    if (rows > ctx->desc.max_tokens)
+        return set_err(ctx, ZR_E_INVALID, "microbatch has %ld tokens (capacity %d)", rows, ctx->desc.max_tokens);
+    const int T = (int)rows;
     if ((size_t)T * V > (size_t)1 << 29)
         return set_err(ctx, ZR_E_INVALID, "verification of %d rows of %d logits: at most 2^29 logits a call", T, V);
     if (zr_status rc = check_ready(ctx)) return rc;
-    std::vector<int> lens(n);
-    for (int s = 0; s < n; ++s) lens[s] = mb->q_len[s] - 1;
     // uniforms [T], drafts [T - n] to the device; tokens [n][out_stride], accepted [n] back
     const size_t in = (size_t)T + (T - n), out = (size_t)n * std::max(out_stride, 0) + n;
+    zr_verify_batch vb{n, lens.data(), nullptr, d_draft_probs, temperature, uniforms};
+    vb.d_drafts = mb->tokens;  // (only looked at for being there)
+    if (zr_status rc = verify_check(ctx, out_tokens, V, &vb, out_tokens, out_stride, accepted)) return rc;
     if (zr_status rc = grow(ctx, &ctx->verify_io, &ctx->verify_io_bytes, 4 * (in + out), "verification staging")) return rc;
     if (4 * (in + out) > ctx->verify_io_host_bytes) {
         if (ctx->verify_io_host) (void)hipHostFree(ctx->verify_io_host);
@@ -2262,18 +2272,21 @@ zr_status zr_forward_verify(zr_context* ctx, const zr_microbatch* mb, const floa
         ZR_HIP(ctx, hipHostMalloc(&ctx->verify_io_host, 4 * (in + out), hipHostMallocDefault));
         ctx->verify_io_host_bytes = 4 * (in + out);
     }
-    uint32_t* h = (uint32_t*)ctx->verify_io_host;
-    uint32_t* d = (uint32_t*)ctx->verify_io;
-    zr_verify_batch vb{n, lens.data(), d + T, d_draft_probs, temperature, (const float*)d};
-    if (zr_status rc = verify_check(ctx, ctx->verify_io, V, &vb, out_tokens, out_stride, accepted)) return rc;
     if (zr_status rc = grow(ctx, (void**)&ctx->row_logits, &ctx->row_logits_bytes, (size_t)4 * T * V, "verification logits"))
         return rc;
     const size_t splitk = gemm_ws_floats(T, V, ctx->desc.hidden, kEpiStore);
     if (splitk > ctx->splitk_ws_floats)
         if (zr_status rc = grow(ctx, (void**)&ctx->row_splitk, &ctx->row_splitk_bytes, 4 * splitk, "split-K workspace")) return rc;
+    StagedMeta* st = ctx->scratch_stage;
+    if (zr_status rc = stage_microbatch(ctx, mb, st)) return rc;
+    // (from here on every way out waits for the stream: the staged host copies are read by it)
+    uint32_t* h = (uint32_t*)ctx->verify_io_host;
+    uint32_t* d = (uint32_t*)ctx->verify_io;
+    vb.d_drafts = d + T;
+    vb.d_uniforms = (const float*)d;
     memcpy(h, uniforms, 4 * (size_t)T);
     for (int s = 0, row = 0; s < n; row += mb->q_len[s], ++s) memcpy(h + T + row - s, mb->tokens + row + 1, 4 * (size_t)lens[s]);
-    ZR_HIP(ctx, hipMemcpyAsync(d, h, 4 * in, hipMemcpyHostToDevice, ctx->stream));
+    hipError_t e = hipMemcpyAsync(d, h, 4 * in, hipMemcpyHostToDevice, ctx->stream);
     // the LM head over all rows may split further than that over last rows
     float* const ws = ctx->splitk_ws;
     const size_t ws_floats = ctx->splitk_ws_floats;
@@ -2281,12 +2294,12 @@ zr_status zr_forward_verify(zr_context* ctx, const zr_microbatch* mb, const floa
         ctx->splitk_ws = ctx->row_splitk;
         ctx->splitk_ws_floats = ctx->row_splitk_bytes / 4;
     }
-    zr_status rc = run_forward(ctx, st, nullptr, nullptr, nullptr, nullptr, true, true);
+    zr_status rc = e == hipSuccess ? run_forward(ctx, st, nullptr, nullptr, nullptr, nullptr, true, true) : ZR_OK;
     ctx->splitk_ws = ws;
     ctx->splitk_ws_floats = ws_floats;
-    if (!rc) rc = launch_verify(ctx, ctx->row_logits, V, &vb, d + in, out_stride, (int*)(d + in + (size_t)n * out_stride));
-    hipError_t e = hipSuccess;
-    if (!rc) e = hipMemcpyAsync(h + in, d + in, 4 * out, hipMemcpyDeviceToHost, ctx->stream);
+    if (e == hipSuccess && !rc)
+        rc = launch_verify(ctx, ctx->row_logits, V, &vb, d + in, out_stride, (int*)(d + in + (size_t)n * out_stride));
+    if (e == hipSuccess && !rc) e = hipMemcpyAsync(h + in, d + in, 4 * out, hipMemcpyDeviceToHost, ctx->stream);
     const hipError_t w = hipStreamSynchronize(ctx->stream);
     if (e == hipSuccess) e = w;
     if (!rc && e != hipSuccess) rc = set_err(ctx, ZR_E_HIP, "forward: %s", hipGetErrorString(e));
