@@ -303,3 +303,37 @@ def test_refusals():
     assert lib.zr_staged_prefix_info(b.st, None) == -1
     other.close()
     b.close()
+
+
+@pytest.mark.parametrize("kv,kv_heads,pages", [("bf16", 8, 70000), ("f32", 8, 35000)])
+def test_pages_past_4_gib(kv, kv_heads, pages):
+    """A layer of more than 2^32 bytes: the same contents at its last pages and, copied, at its first."""
+    ctx = DeviceContext(ModelGeometry(4 * 8 * 128, 32, kv_heads, 1, 32, 64), kv_dtype=kv, max_tokens=64, max_seqs=8,
+                        max_pages_per_seq=128, split_activations=True)
+    ctx.create_kv_pool(pages)
+    assert ctx.kv_pool_bytes() > 1 << 32
+    ctx.check(ctx.lib.zr_kv_pool_fill_normal(ctx.h, 3, 1.0))
+    rng = np.random.default_rng(5)
+    n, shared, own = 6, 90, 20
+    low = rng.permutation(shared + n * own).astype(np.int32)
+    high = (pages - 1 - rng.permutation(shared + n * own)).astype(np.int32)
+    assert (int(high.min()) + 1) * (ctx.kv_pool_bytes() // pages) > 1 << 32
+    ctx.copy_pages(high, low)
+    q = (rng.standard_normal((n, 32 * 128)) * 1.3).astype(np.float32)
+    d_q, d_o = DeviceBuffer.from_numpy(ctx, q), DeviceBuffer(ctx, q.nbytes)
+    out = []
+    for ids in (high, low):
+        tables = np.array([np.concatenate([ids[:shared], ids[shared + i * own:shared + (i + 1) * own]]) for i in range(n)], np.int32)
+        ones, before, zero = np.ones(n, np.int32), np.full(n, (shared + own) * 16 - 5, np.int32), np.zeros(n, np.int32)
+        mb = _lib.Microbatch(n, i32p(ones), i32p(before), i32p(before), i32p(zero), i32p(tables), shared + own, None)
+        st, info = C.c_void_p(), _lib.PrefixInfo()
+        ctx.check(ctx.lib.zr_stage(ctx.h, C.byref(mb), C.byref(st)))
+        ctx.check(ctx.lib.zr_staged_prefix_info(st.value, C.byref(info)))
+        assert info.segments == 1 and info.sequences == n
+        ctx.check(ctx.lib.zr_attention(ctx.h, st.value, 0, d_q.ptr, d_o.ptr))
+        out.append(d_o.download(np.float32, q.shape))
+        ctx.lib.zr_staged_destroy(st.value)
+    assert np.isfinite(out[0]).all()
+    np.testing.assert_array_equal(out[0], out[1])
+    assert np.std(out[0]) > 1e-3
+    ctx.close()

@@ -7,7 +7,8 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from mesh_amd import BackendMicrobatchExecutor, DecodeMicrobatchRequest, DecodePipeline
+from mesh_amd import BackendMicrobatchExecutor, DecodeMicrobatchRequest, DecodePipeline, DeviceBuffer
+from mesh_amd._lib import PrefixInfo
 from tests.test_gpu_fork_pages import model_context
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +115,62 @@ def test_sessions_that_leave_the_shared_start_go_on_by_themselves(monkeypatch):
     assert steps(again, first, 12, False) == want
     same_cache(alone, again)
     ctx.close()
+
+
+def test_a_captured_shared_step_replays_its_logits():
+    ctx = model_context("bf16", 8, 2, 128, pages=300)
+    lib, n = ctx.lib, 6
+    parent = prompt_of(ctx, 260)
+    forks = [parent.fork() for _ in range(n)]
+    other = prompt_of(ctx, 40, 7)
+    arr = (C.c_void_p * n)(*[b.h for b in forks])
+    st, g = C.c_void_p(), C.c_void_p()
+    tokens = np.arange(3, 3 + n, dtype=np.uint32)
+    ones = np.ones(n, np.int32)
+    ctx.check(lib.zrh_stage_mixed(C.cast(arr, C.POINTER(C.c_void_p)), n, ones.ctypes.data_as(C.POINTER(C.c_int)),
+                                  tokens.ctypes.data_as(C.POINTER(C.c_uint32)), C.byref(st)))
+    info = PrefixInfo()
+    ctx.check(lib.zr_staged_prefix_info(st.value, C.byref(info)))
+    assert (info.segments, info.sequences, info.rows) == (1, n, n)
+    logits = DeviceBuffer(ctx, 4 * n * 512)
+    other.decode_step(1)  # (grows what it needs before the capture)
+    ctx.check(lib.zr_forward_staged_async(ctx.h, st.value, None, None, logits.ptr))
+    ctx.check(lib.zr_synchronize(ctx.h))
+    want = logits.download(np.float32, (n, 512))
+    assert np.isfinite(want).all()
+    ctx.check(lib.zr_graph_capture_staged(ctx.h, st.value, None, None, logits.ptr, C.byref(g)))
+    for _ in range(4):
+        logits.upload(np.full((n, 512), np.nan, np.float32))
+        ctx.check(lib.zr_graph_launch(ctx.h, g.value))
+        ctx.check(lib.zr_synchronize(ctx.h))
+        np.testing.assert_array_equal(logits.download(np.float32, (n, 512)), want)
+        other.decode_step(2)  # the program's own eager work between replays
+    lib.zr_graph_destroy(g.value)
+    lib.zr_staged_destroy(st.value)
+    ctx.close()
+
+
+def test_two_contexts_at_once():
+    """Each context has its own stream and workspaces: interleaved steps are those of each alone."""
+    rng = np.random.default_rng(11)
+    ctxs = [model_context(kv, 4, 2, 64, pages=300) for kv in ("bf16", "f32")]
+    parents = [prompt_of(c, 150 + 30 * i) for i, c in enumerate(ctxs)]
+    first = rng.integers(0, 512, 4).tolist()
+    alone = []
+    for p in parents:
+        forks = [p.fork() for _ in range(4)]
+        alone.append(steps(forks, first, 10, False))
+    forks = [[p.fork() for _ in range(4)] for p in parents]
+    pipes = [DecodePipeline(f, first) for f in forks]  # (both streams run while the host goes on)
+    got = [[], []]
+    for _ in range(10):
+        for out, p in zip(got, pipes):
+            t = p.step()
+            if t is not None:
+                out.append(list(t))
+    for out, p in zip(got, pipes):
+        out.append(list(p.finish()))
+        p.close()
+    assert got == alone
+    for c in ctxs:
+        c.close()

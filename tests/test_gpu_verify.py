@@ -259,3 +259,26 @@ def test_refusals(ctx):
         verify_device(ctx, np.zeros((2, 4), np.float32), [[1], []], [1.0, 1.0], np.zeros(2))
     with pytest.raises(ZrError):
         verify_device(ctx, np.zeros((2, 4), np.float32), [[1]], [1.0], np.zeros(2), np.zeros((1, 5)))
+
+
+@pytest.mark.parametrize("cols", [2048, 5001])
+@pytest.mark.parametrize("x_off,q_off", [(4, 0), (0, 4), (4, 8), (12, 12)])
+def test_rows_at_any_alignment(ctx, cols, x_off, q_off):
+    rng = np.random.default_rng(cols + x_off)
+    lens = [3, 1, 2]
+    temps = np.array([0.8, 1.0, 0.0], np.float32)
+    logits, drafts, u, q = problem(rng, cols, lens, temps, False)
+    ln = np.array(lens, np.int32)
+    y, du = DeviceBuffer.from_numpy(ctx, np.array([t for d in drafts for t in d], np.uint32)), DeviceBuffer.from_numpy(ctx, u)
+    pad = [DeviceBuffer.from_numpy(ctx, np.concatenate([np.full(o // 4, np.inf, np.float32), np.ravel(a)]))
+           for o, a in ((x_off, logits), (q_off, q))]
+    out, acc = DeviceBuffer(ctx, 4 * 3 * 9), DeviceBuffer(ctx, 12)
+    out.upload(np.full(27, 7, np.uint32))
+    vb = _lib.VerifyBatch(3, ln.ctypes.data_as(_lib.c_int_p), y.ptr, pad[1].ptr + q_off, temps.ctypes.data_as(_lib.c_f32_p),
+                          du.ptr)
+    ctx.check(ctx.lib.zr_verify(ctx.h, pad[0].ptr + x_off, cols, C.byref(vb), out.ptr, 9, acc.ptr))
+    a, t = acc.download(np.int32, (3,)), out.download(np.uint32, (3, 9))
+    want = expect(logits, drafts, temps, u, q)
+    assert a.tolist() == want[1]
+    for s in range(3):
+        assert t[s, :a[s] + 1].tolist() == want[0][s] and np.all(t[s, a[s] + 1:] == 0xffffffff)
