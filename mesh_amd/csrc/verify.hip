@@ -194,9 +194,23 @@ template <int N> __device__ inline int seq_of(const VerifyArgs<N>& v, int n, int
     return lo;
 }
 
+// Four columns from c on; the ones past the row's end are `none`.  Rows of an odd
+// length start at any multiple of 4 bytes: so do these 16-byte loads.
+struct __attribute__((packed, aligned(4))) Four {
+    float x, y, z, w;
+};
+__device__ inline float4 four(const float* x, int c) {
+    const Four f = *(const Four*)(x + c);
+    return make_float4(f.x, f.y, f.z, f.w);
+}
+__device__ inline float4 four_to(const float* x, int c, int cols, float none) {
+    if (c + 4 <= cols) return four(x, c);
+    return make_float4(c < cols ? x[c] : none, c + 1 < cols ? x[c + 1] : none, c + 2 < cols ? x[c + 2] : none, none);
+}
+
 // A workgroup of 4 waves takes one chunk of 1024 E columns of one row; every
 // load of a lane goes out before the first is used.
-template <int E, bool VEC, int N>
+template <int E, int N>
 __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyArgs<N> v, int n) {
     __shared__ float sm[4];
     __shared__ int sat[4];
@@ -205,19 +219,12 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyA
     const int c0 = ch * b.chunk, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* x = b.logits + (size_t)row * b.cols;
     float4 d[E];
+    if (c0 + b.chunk <= b.cols) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int c = c0 + (e * 256 + tid) * 4;
-        const float none = -INFINITY;
-        if constexpr (VEC) {
-            d[e] = c < b.cols ? *(const float4*)(x + c) : make_float4(none, none, none, none);
-        } else {  // rows that are not 16-byte aligned: the same columns in another order (c0 + 256 of a lane's four apart)
-            const int c1 = c0 + e * 1024 + tid;
-            d[e].x = c1 < b.cols ? x[c1] : none;
-            d[e].y = c1 + 256 < b.cols ? x[c1 + 256] : none;
-            d[e].z = c1 + 512 < b.cols ? x[c1 + 512] : none;
-            d[e].w = c1 + 768 < b.cols ? x[c1 + 768] : none;
-        }
+        for (int e = 0; e < E; ++e) d[e] = four(x, c0 + (e * 256 + tid) * 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] = four_to(x, c0 + (e * 256 + tid) * 4, b.cols, -INFINITY);
     }
     const float t = v.temp[seq_of(v, n, row)];  // (behind the loads' issue: a chain of scalar loads)
     float m = -INFINITY;
@@ -227,7 +234,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyBufs b, VerifyA
         const float f[4] = {d[e].x, d[e].y, d[e].z, d[e].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int c = VEC ? c0 + (e * 256 + tid) * 4 + j : c0 + e * 1024 + tid + 256 * j;
+            const int c = c0 + (e * 256 + tid) * 4 + j;
             if (f[j] > m) {  // (a lane's columns ascend: the first of equals stays)
                 m = f[j];
                 at = c;
@@ -325,7 +332,7 @@ template <int N> __device__ inline Decision decide(const VerifyBufs& b, const Ve
 
 // A workgroup takes `per` chunks of one sequence's emission row in turn: as many as
 // leave no more workgroups than the chip holds at once, for each has the tests to do first.
-template <bool VEC, int N>
+template <int N>
 __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyArgs<N> v, int per, int groups) {
     __shared__ double ss[2][3][4];
     constexpr int E = kRestChunk / 256;
@@ -341,33 +348,23 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyAr
         const int c0 = ch * kRestChunk, buf = ch & 1;
         float x[E], q[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] = -INFINITY;
-            q[e] = 0.0f;
-        }
-        if constexpr (VEC) {
-#pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                const int c = c0 + e * 256 + tid * 4;
-                if (c < b.cols) {
-                    *(float4*)(x + e) = *(const float4*)(xr + c);
-                    if (qr) *(float4*)(q + e) = *(const float4*)(qr + c);
-                }
+        for (int e = 0; e < E; e += 4) {
+            const int c = c0 + e * 256 + tid * 4;
+            float4 xv, qv = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (c0 + kRestChunk <= b.cols) {
+                xv = four(xr, c);
+                if (qr) qv = four(qr, c);
+            } else {
+                xv = four_to(xr, c, b.cols, -INFINITY);
+                if (qr) qv = four_to(qr, c, b.cols, 0.0f);
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int c = c0 + e * 256 + tid;
-                if (c < b.cols) {
-                    x[e] = xr[c];
-                    if (qr) q[e] = qr[c];
-                }
-            }
+            x[e] = xv.x, x[e + 1] = xv.y, x[e + 2] = xv.z, x[e + 3] = xv.w;
+            q[e] = qv.x, q[e + 1] = qv.y, q[e + 2] = qv.z, q[e + 3] = qv.w;
         }
         double w = 0.0, wa = 0.0, qa = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int c = VEC ? c0 + (e / 4) * 1024 + tid * 4 + (e & 3) : c0 + e * 256 + tid;
+            const int c = c0 + (e / 4) * 1024 + tid * 4 + (e & 3);
             const double we = weight.inf ? (x[e] == d.m ? 1.0 : 0.0) : weight(x[e]);
             const float qe = fmaxf(q[e], 0.0f);
             w += we;
@@ -505,8 +502,7 @@ __global__ __launch_bounds__(kEmitThreads) void verify_emit_kernel(VerifyBufs b)
 
 // The pass over all logits and that over the emission rows of m <= N sequences.
 template <int N>
-void launch_passes(zr_context* ctx, const VerifyBufs& b, const int* draft_len, const float* temperature, int m, int e,
-                   bool vec, bool rest_vec) {
+void launch_passes(zr_context* ctx, const VerifyBufs& b, const int* draft_len, const float* temperature, int m, int e) {
     VerifyArgs<N> v;
     int r = 0;
     for (int s = 0; s < N; ++s) {
@@ -519,16 +515,13 @@ void launch_passes(zr_context* ctx, const VerifyBufs& b, const int* draft_len, c
         hipLaunchKernelGGL(kernel, dim3(r * b.chunks), dim3(256), 0, ctx->stream, b, v, m);
     };
     switch (e) {
-        case 1: if (vec) stats(verify_stats_kernel<1, true, N>); else stats(verify_stats_kernel<1, false, N>); break;
-        case 2: if (vec) stats(verify_stats_kernel<2, true, N>); else stats(verify_stats_kernel<2, false, N>); break;
-        case 4: if (vec) stats(verify_stats_kernel<4, true, N>); else stats(verify_stats_kernel<4, false, N>); break;
-        default: if (vec) stats(verify_stats_kernel<8, true, N>); else stats(verify_stats_kernel<8, false, N>); break;
+        case 1: stats(verify_stats_kernel<1, N>); break;
+        case 2: stats(verify_stats_kernel<2, N>); break;
+        case 4: stats(verify_stats_kernel<4, N>); break;
+        default: stats(verify_stats_kernel<8, N>); break;
     }
     const int per = (m * b.rest_chunks + 2047) / 2048, groups = (b.rest_chunks + per - 1) / per;
-    auto rest = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
-    };
-    if (rest_vec) rest(verify_rest_kernel<true, N>); else rest(verify_rest_kernel<false, N>);
+    hipLaunchKernelGGL(verify_rest_kernel<N>, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
 }
 
 }  // namespace
@@ -580,14 +573,12 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
         b.out = d_out + (size_t)s0 * out_stride;
         b.out_stride = out_stride;
         b.accepted = d_accepted + s0;
-        const bool vec = cols % 4 == 0 && ((uintptr_t)d_logits & 15) == 0;
         const int *lens = vb->draft_len + s0;
         const float* temps = vb->temperature + s0;
-        const bool rest_vec = vec && ((uintptr_t)vb->d_draft_probs & 15) == 0;
         if (m <= kFewSeqs)
-            launch_passes<kFewSeqs>(ctx, b, lens, temps, m, e, vec, rest_vec);
+            launch_passes<kFewSeqs>(ctx, b, lens, temps, m, e);
         else
-            launch_passes<kSeqs>(ctx, b, lens, temps, m, e, vec, rest_vec);
+            launch_passes<kSeqs>(ctx, b, lens, temps, m, e);
         ZR_LAUNCH_CHECK(ctx);
         hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(kEmitThreads), 0, ctx->stream, b);
         ZR_LAUNCH_CHECK(ctx);
