@@ -320,7 +320,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     if (stride <= 0 || stride > ctx->desc.max_pages_per_seq)
         return set_err(ctx, ZR_E_INVALID, "block table stride %d outside 1..%d", stride, ctx->desc.max_pages_per_seq);
     if (!ctx->kv_pool) return set_err(ctx, ZR_E_INVALID, "KV pool not created");
-    int total_q = 0, max_kv = 0;
+    int total_q = 0, max_kv = 0, max_page = 0;
     for (int s = 0; s < S; ++s) {
         const int ql = mb->q_len[s], kb = mb->kv_before[s], fo = mb->first_offset[s];
         if (ql <= 0) return set_err(ctx, ZR_E_INVALID, "sequence %d has q_len %d", s, ql);
@@ -338,6 +338,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
             if (id < 0 || id >= ctx->n_pages)
                 return set_err(ctx, ZR_E_INVARIANT, "sequence %d page slot %ld holds page %d outside pool of %d", s, p,
                                id, ctx->n_pages);
+            max_page = std::max(max_page, id);
         }
         total_q += ql;
         max_kv = std::max(max_kv, kb + ql);
@@ -354,6 +355,7 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     const int blob_stride = fixed ? fixed->stride : stride;
     st->ctx = ctx;
     st->page_epoch = ctx->page_epoch;
+    st->max_page = max_page;
     st->num_seqs = S;
     st->total_q = total_q;
     st->stride = blob_stride;
@@ -1213,10 +1215,13 @@ void zr_staged_destroy(zr_staged* s) {
     delete st;
 }
 
-// A microbatch staged before a compaction names pages that have moved.
-static zr_status pages_current(zr_context* ctx, uint64_t page_epoch) {
+// A microbatch staged before a compaction names pages that have moved; one staged
+// before the pool was re-created may name pages that it no longer has.
+static zr_status pages_current(zr_context* ctx, uint64_t page_epoch, int max_page) {
     if (page_epoch != ctx->page_epoch)
         return set_err(ctx, ZR_E_INVALID, "staged before the pool's pages were compacted: stage it again");
+    if (max_page >= ctx->n_pages)
+        return set_err(ctx, ZR_E_INVALID, "staged with page %d of another pool, this one has %d", max_page, ctx->n_pages);
     return ZR_OK;
 }
 
@@ -1224,7 +1229,7 @@ zr_status zr_forward_staged_async(zr_context* ctx, zr_staged* s, const uint32_t*
                                   float* d_out_logits) {
     StagedMeta* st = (StagedMeta*)s;
     if (!ctx || !st || st->ctx != ctx) return set_global_err(ZR_E_INVALID, "staged microbatch of another context");
-    if (zr_status rc = pages_current(ctx, st->page_epoch)) return rc;
+    if (zr_status rc = pages_current(ctx, st->page_epoch, st->max_page)) return rc;
     return run_forward(ctx, st, d_tokens, d_out_tokens, d_out_logits, nullptr, false);
 }
 
@@ -1254,6 +1259,7 @@ struct zr_graph {
     uint64_t buffer_epoch = 0; // the context's buffer epoch at capture
     uint64_t staged_id = 0;    // the staged microbatch the graph replays
     uint64_t page_epoch = 0;   // ... and the page ids it was staged with
+    int max_page = 0;
 };
 
 zr_status zr_graph_capture_staged(zr_context* ctx, zr_staged* s, const uint32_t* d_tokens, uint32_t* d_out_tokens,
@@ -1261,7 +1267,7 @@ zr_status zr_graph_capture_staged(zr_context* ctx, zr_staged* s, const uint32_t*
     StagedMeta* st = (StagedMeta*)s;
     if (!ctx || !st || !out) return set_global_err(ZR_E_INVALID, "null argument");
     if (st->ctx != ctx) return set_err(ctx, ZR_E_INVALID, "staged microbatch of another context");
-    if (zr_status rc = pages_current(ctx, st->page_epoch)) return rc;
+    if (zr_status rc = pages_current(ctx, st->page_epoch, st->max_page)) return rc;
     // HIP events recorded by graph nodes do not time (hipEventElapsedTime
     // reports an invalid handle for them), so timing stays eager-only
     if (ctx->timing.enabled) return set_err(ctx, ZR_E_INVALID, "graph capture with per-class timing on");
@@ -1293,6 +1299,7 @@ zr_status zr_graph_capture_staged(zr_context* ctx, zr_staged* s, const uint32_t*
     g->buffer_epoch = ctx->buffer_epoch;
     g->staged_id = st->id;
     g->page_epoch = st->page_epoch;
+    g->max_page = st->max_page;
     *out = g;
     return ZR_OK;
 }
@@ -1305,7 +1312,7 @@ zr_status zr_graph_launch(zr_context* ctx, zr_graph* g) {
                        "graph captured before a workspace, the KV pool or weights were reallocated: capture it again");
     if (std::find(ctx->live_staged.begin(), ctx->live_staged.end(), g->staged_id) == ctx->live_staged.end())
         return set_err(ctx, ZR_E_INVALID, "the graph's staged microbatch was destroyed: stage and capture again");
-    if (zr_status rc = pages_current(ctx, g->page_epoch)) return rc;
+    if (zr_status rc = pages_current(ctx, g->page_epoch, g->max_page)) return rc;
     ZR_HIP(ctx, hipGraphLaunch(g->exec, ctx->stream));
     if (g->token_check) ctx->token_check_pending = true;
     ctx->last_logits = true;
@@ -1672,7 +1679,7 @@ zr_status zr_pack(zr_context* ctx, const zr_microbatch* mb, int* cu_q, int* cu_k
 // staged by another context is refused before anything launches.
 static zr_status staged_for(zr_context* ctx, const StagedMeta* st) {
     if (st->ctx != ctx) return set_err(ctx, ZR_E_INVALID, "staged microbatch of another context");
-    return pages_current(ctx, st->page_epoch);
+    return pages_current(ctx, st->page_epoch, st->max_page);
 }
 
 zr_status zr_rope_kv_write(zr_context* ctx, zr_staged* s, int layer, const float* d_qkv, float* d_q_out, int rope) {

@@ -317,6 +317,7 @@ struct StagedMeta {
     zr_context* ctx = nullptr;
     uint64_t id = 0;          // zr_stage handle id (zr_context::live_staged)
     uint64_t page_epoch = 0;  // zr_context::page_epoch when staged
+    int max_page = 0;         // the highest page id it names
     int num_seqs = 0, total_q = 0, stride = 0;
     int max_kv = 0;           // max kv_after over sequences
     int n_attn_items = 0;     // attention work items (per kv head)

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from mesh_amd import DeviceBuffer, DeviceContext, ModelGeometry, _lib
+from mesh_amd._lib import ZrError
 from tests.gpu_util import f32p, i32p
 
 pytestmark = pytest.mark.gpu
@@ -337,3 +338,14 @@ def test_pages_past_4_gib(kv, kv_heads, pages):
     np.testing.assert_array_equal(out[0], out[1])
     assert np.std(out[0]) > 1e-3
     ctx.close()
+
+
+def test_a_smaller_pool_refuses_what_named_pages_it_has_not():
+    p = Batch("bf16", 4, 2, 64, [(list(range(12)) + [12 + i], 0, 195, 1) for i in range(3)])
+    p.attend()
+    p.ctx.check(p.ctx.lib.zr_kv_pool_create(p.ctx.h, 14))
+    with pytest.raises(ZrError, match="page 14 of another pool, this one has 14"):
+        p.attend()
+    p.ctx.check(p.ctx.lib.zr_kv_pool_create(p.ctx.h, 15))
+    assert np.all(p.attend() == 0)  # (the same page ids, in the new pool)
+    p.ctx.close()
