@@ -272,3 +272,86 @@ def test_forward_refusals():
     assert ctx.lib.zr_forward_verify(ctx.h, None, None, None, None, None, 1, None) == -1
     assert ctx.lib.zr_forward_verify(None, None, None, None, None, None, 1, None) == -1
     ctx.close()
+
+
+@pytest.mark.parametrize("kv,kv_heads,d", [("f32", 1, 64), ("bf16", 2, 128)])
+@pytest.mark.parametrize("seed", [0, 1])
+def test_any_program_of_forks_steps_drafts_and_compactions(kv, kv_heads, d, seed):
+    """Random calls; in the end every window holds the keys and values of its own tokens, as a session
+    that was prefilled with them has them."""
+    from mesh_amd import DecodeMicrobatchRequest
+    ctx = model_context(kv, 4, kv_heads, d, pages=220)
+    rng = np.random.default_rng(seed)
+    live = []  # [session, its tokens]
+
+    def some(n=None):
+        n = int(rng.integers(1, min(len(live), 12) + 1)) if n is None else n
+        return [live[i] for i in rng.permutation(len(live))[:n]]
+
+    for step in range(150):
+        what = rng.choice(["new", "fork", "fork", "step", "step", "step", "verify", "verify", "chunk", "truncate", "close",
+                           "compact"])
+        if what == "new" or not live:
+            if len(live) < 14:
+                tokens = rng.integers(0, VOCAB, int(rng.integers(1, 120))).tolist()
+                b = ctx.new_backend()
+                b.prefill(tokens)
+                live.append([b, tokens])
+        elif what == "fork" and len(live) < 14:
+            b, tokens = some(1)[0]
+            live.append([b.fork(), list(tokens)])
+        elif what == "step":
+            part = some()
+            for _ in range(int(rng.integers(1, 7))):  # (as many as replay)
+                toks = rng.integers(0, VOCAB, len(part)).tolist()
+                BackendMicrobatchExecutor.decode_step_batch(
+                    [DecodeMicrobatchRequest("", t, s[0]) for t, s in zip(toks, part)])
+                for t, s in zip(toks, part):
+                    s[1].append(t)
+        elif what == "verify":
+            part = some(min(len(live), 10))
+            reqs = []
+            for s in part:
+                k = int(rng.integers(0, 6))
+                reqs.append(Request("", int(rng.integers(0, VOCAB)), rng.integers(0, VOCAB, k).tolist(), s[0],
+                                    temperature=8.0, uniforms=(rng.random(k + 1) * 1e-3).tolist()))
+            for s, r, (tokens, a) in zip(part, reqs, verify(reqs)):
+                assert tokens[:a] == r.drafts[:a] and len(tokens) == a + 1
+                s[1] += [r.token] + r.drafts[:a]
+        elif what == "chunk":
+            part = some(min(len(live), 4))
+            chunks = [rng.integers(0, VOCAB, int(rng.integers(1, 32))).tolist() for _ in part]
+            BackendMicrobatchExecutor.forward_mixed([s[0] for s in part], chunks, want_logits=False)
+            for c, s in zip(chunks, part):
+                s[1] += c
+        elif what == "truncate":
+            s = some(1)[0]
+            n = int(rng.integers(0, min(len(s[1]), 40)))
+            s[0].truncate(n)
+            del s[1][len(s[1]) - n:]
+        elif what == "close" and len(live) > 3:
+            s = some(1)[0]
+            live.remove(s)
+            s[0].close()
+        elif what == "compact":
+            ctx.compact_pages()
+        while ctx.free_pages < 60:
+            live.pop(int(rng.integers(0, len(live))))[0].close()
+        for b, tokens in live:
+            assert b.sequence_position() == b.cache_seq_len() == len(tokens)
+    for b, tokens in live:
+        got = b.export_kv_cache()
+        own = ctx.new_backend()
+        own.prefill(tokens)
+        want = own.export_kv_cache()
+        own.close()
+        # Other batches form their sums in other orders.  Activations enter the products as hi + lo
+        # bf16, 16 bits: where the last f32 bits differ, lo may fall a step apart, 2^-16 of x.  A key
+        # of layer 1 sums 256 of them (x of order 1, w of 0.05: 16 * 0.05 * 2^-16 = 1.2e-5 in the
+        # mean square if all did), and what reached x through layer 0's three products is of the same
+        # size, so six deviations are 1e-4 and a little.  A bf16 pool adds a step of a value on a tie,
+        # 2^-7 of it at most, and its weight in the layer above.  A wrong row is off by order 1.
+        rtol, atol = (2.0 ** -7, 2e-3) if kv == "bf16" else (0, 2e-4)
+        np.testing.assert_allclose(got.keys, want.keys, rtol=rtol, atol=atol)
+        np.testing.assert_allclose(got.values, want.values, rtol=rtol, atol=atol)
+    ctx.close()
