@@ -174,3 +174,33 @@ def test_two_contexts_at_once():
     assert got == alone
     for c in ctxs:
         c.close()
+
+
+@pytest.mark.parametrize("rows", [77, 80, 95])
+def test_a_session_forked_inside_a_pipeline(rows):
+    ctx = model_context("bf16", 4, 2, 64, pages=300)
+    parent = prompt_of(ctx, rows)
+    first = [4, 5, 6]
+    eager, piped = ([parent.fork() for _ in range(3)] for _ in range(2))
+    want = steps(eager, first, 20, True)
+    p = DecodePipeline(piped, first)
+    got, children = [], []
+    for i in range(20):
+        t = p.step()
+        if t is not None:
+            got.append(list(t))
+        if i % 6 == 2:  # with this step in flight
+            children.append((piped[1].fork(), i + 1))
+            assert children[-1][0].cache_seq_len() == rows + i + 1
+        if i % 6 == 4:  # a child writes beside the pipeline's own writes
+            children[-1][0].decode_step(9)
+    got.append(list(p.finish()))
+    p.close()
+    assert got == want
+    same_cache(eager, piped)
+    whole = eager[1].export_kv_cache()
+    for child, n in children:
+        c = child.export_kv_cache()
+        np.testing.assert_array_equal(c.keys[:, :rows + n], whole.keys[:, :rows + n])
+        np.testing.assert_array_equal(c.values[:, :rows + n], whole.values[:, :rows + n])
+    ctx.close()
