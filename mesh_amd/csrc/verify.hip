@@ -362,19 +362,27 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyAr
             q[e] = qv.x, q[e + 1] = qv.y, q[e + 2] = qv.z, q[e + 3] = qv.w;
         }
         double w = 0.0, wa = 0.0, qa = 0.0;
+        if (qr) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int c = c0 + (e / 4) * 1024 + tid * 4 + (e & 3);
-            const double we = weight.inf ? (x[e] == d.m ? 1.0 : 0.0) : weight(x[e]);
-            const float qe = fmaxf(q[e], 0.0f);
-            w += we;
-            const bool in = qr ? (float)we > qe * d.z : (uint32_t)c != d.out;
-            wa += in ? we : 0.0;
-            qa += (double)(in ? qe : 0.0f);
+            for (int e = 0; e < E; ++e) {
+                const double we = weight.inf ? (x[e] == d.m ? 1.0 : 0.0) : weight(x[e]);
+                const float qe = fmaxf(q[e], 0.0f);
+                w += we;
+                const bool in = (float)we > qe * d.z;
+                wa += in ? we : 0.0;
+                qa += (double)(in ? qe : 0.0f);
+            }
+            wa = wave_sum(wa);
+            qa = wave_sum(qa);
+        } else {  // p, without a certain draft's own column (alone in weighing, it is drawn as the largest)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float xe = (uint32_t)(c0 + (e / 4) * 1024 + tid * 4 + (e & 3)) == d.out ? -INFINITY : x[e];
+                w += weight.inf ? (xe == d.m ? 1.0 : 0.0) : weight(xe);
+            }
         }
         w = wave_sum(w);
-        wa = wave_sum(wa);
-        qa = wave_sum(qa);
+        if (!qr) wa = w;
         if ((tid & 63) == 0) {
             ss[buf][0][tid >> 6] = w;
             ss[buf][1][tid >> 6] = wa;
