@@ -25,13 +25,13 @@
 // of 32000, measured one after another):
 //   verify_stats_kernel  one pass over all logits: per chunk of a row its largest
 //                        logit, the first place of it, and the f32 sum of weights
-//                        relative to it.  HBM bound (27.6: 6 TB/s; 3.6).
+//                        relative to it.  HBM bound (27.5: 6 TB/s; 3.6).
 //   verify_rest_kernel   the tests, then per chunk of the emission row in f64:
 //                        W = sum w, and over A = {w > q Z} the sums of w and q.
 //                        The rest's weight is then W_A - Q_A Z with the f64 Z =
 //                        sum W: a column that the f32 Z puts on the wrong side of A
 //                        weighs below 1e-7 of itself.  Bound by f64 rates and by the
-//                        tests' chain of loads before it (21.2; 6.2).
+//                        tests' chain of loads before it (20.8; 6.0).
 //   verify_emit_kernel   the crossing's chunk by the chunks' sums, then its place in
 //                        the chunk, which is weighed again: a chain of latencies
 //                        (5.1; 5.2)
