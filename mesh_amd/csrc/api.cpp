@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cstdlib>
+#include <map>
 
 #include "zr_internal.h"
 
@@ -583,6 +584,28 @@ zr_status stage_microbatch(zr_context* ctx, const zr_microbatch* mb, StagedMeta*
     std::stable_sort(st->h_order.begin(), st->h_order.end(), [&](int x, int y) {
         return st->h_items[x].z - st->h_items[x].y > st->h_items[y].z - st->h_items[y].y;
     });
+    // ... and, beside shared segments, the tiles of one sequence (several where rows x q
+    // heads pass 16 columns) one behind the other on one XCD, which takes every eighth
+    // record: they read the same pages (48 x 5 rows of 4 heads: 39.7 -> 38.4 us)
+    if (!segments.empty() && n_decode_tiles > S) {
+        std::vector<std::vector<int>> runs;  // items of one sequence and page range
+        std::map<std::pair<int, int>, size_t> run_of;
+        for (int item : st->h_order) {
+            const int4 it = st->h_items[item];
+            const auto at = run_of.emplace(std::make_pair(st->h_tiles[it.x].x, it.y), runs.size());
+            if (at.second) runs.emplace_back();
+            runs[at.first->second].push_back(item);
+        }
+        size_t n = 0;
+        for (size_t b = 0; b < runs.size(); b += 8) {
+            const size_t e = std::min(b + 8, runs.size()), end = n;
+            size_t left = 0;
+            for (size_t k = b; k < e; ++k) left += runs[k].size();
+            for (size_t i = 0; n < end + left; ++i)
+                for (size_t k = b; k < e; ++k)
+                    if (i < runs[k].size()) st->h_order[n++] = runs[k][i];
+        }
+    }
     // tiles whose splits need the merge kernel (every prefill group tile has several)
     st->h_merge.clear();
     for (int t = 0; t < st->n_tiles; ++t)
