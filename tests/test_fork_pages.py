@@ -330,3 +330,39 @@ def test_sessions_of_a_destroyed_pool_refuse_rows():
     assert LIB.zrh_kv_reserve(b.h, 1) == -1
     assert "pool was destroyed" in LIB.zr_global_last_error().decode()
     b.close()
+
+
+def test_a_verified_step_that_cannot_run_leaves_every_session_as_it_was():
+    """Without a device the step is assembled, refused and rolled back, shared pages and copies included."""
+    m = Model(8, max_seq=64)
+    a = m.new()
+    m.reserve(a, 40)
+    c, tight = m.new(), m.new(max_seq=41)
+    for s in (c, tight):
+        _lib.check(fork(m.sessions[a], m.sessions[s]))
+        m.rows[s] = list(m.rows[a])
+    i32, u32, f32 = (lambda x: x.ctypes.data_as(_lib.c_int_p)), (lambda x: x.ctypes.data_as(_lib.c_u32_p)), \
+        (lambda x: x.ctypes.data_as(_lib.c_f32_p))
+
+    def step(who, drafts, stride=300):
+        n = len(who)
+        h = (C.c_void_p * n)(*[m.sessions[s].h for s in who])
+        k, toks = np.array(drafts, np.int32), np.zeros(max(1, sum(drafts) + n), np.uint32)
+        u, t = np.zeros(toks.size, np.float32), np.zeros(n, np.float32)
+        out, acc = np.zeros(n * 300, np.uint32), np.full(n, -7, np.int32)
+        rc = LIB.zrh_verify_batch(C.cast(h, C.POINTER(C.c_void_p)), n, i32(k), u32(toks), f32(t), f32(u), None, u32(out),
+                                  stride, i32(acc))
+        assert np.all(acc == -7) and not out.any()
+        return rc
+
+    before = [m.places(s) for s in (a, c, tight)]
+    free = LIB.zrh_pool_free_pages(m.pool)
+    for who, drafts, kw in (([a, c], [2, 3], {}),          # both would take copies of the last page
+                            ([a, c], [20, 20], {}),        # more pages than the pool has
+                            ([a, tight], [2, 1], {}),      # the second window would slide
+                            ([a, a], [1, 1], {}),
+                            ([a], [256], {}), ([a], [-1], {}), ([a, c], [1, 4], dict(stride=4))):
+        assert step(who, drafts, **kw) < 0, (who, drafts)
+        assert [m.places(s) for s in (a, c, tight)] == before and LIB.zrh_pool_free_pages(m.pool) == free
+        m.check()
+    m.close()

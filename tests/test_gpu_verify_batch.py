@@ -5,7 +5,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from mesh_amd import BackendMicrobatchExecutor, DeviceBuffer, DeviceContext, ModelGeometry
+from mesh_amd import BackendMicrobatchExecutor, DecodeMicrobatchRequest, DeviceBuffer, DeviceContext, ModelGeometry
 from mesh_amd import VerifyMicrobatchRequest as Request
 from mesh_amd._lib import Microbatch, ZrError
 from tests.gpu_util import i32p
@@ -85,7 +85,6 @@ def test_forks_with_drafts_emit_the_greedy_path(kv, heads, kv_heads, d, rows):
             last[i] = t[-1]
             assert forks[i].sequence_position() == rows + done[i] == forks[i].cache_seq_len()
     # ordinary steps go on from there, in eager and replayed microbatches
-    from mesh_amd import DecodeMicrobatchRequest
     for step in range(5):
         out = BackendMicrobatchExecutor.decode_step_batch(
             [DecodeMicrobatchRequest(str(i), last[i], f) for i, f in enumerate(forks)])
@@ -237,7 +236,6 @@ def test_sampling_after_a_verification_needs_a_forward():
                                              one.ctypes.data_as(C.POINTER(C.c_float)),
                                              seed.ctypes.data_as(C.POINTER(C.c_uint64)),
                                              out.ctypes.data_as(C.POINTER(C.c_uint32)))
-    from mesh_amd import DecodeMicrobatchRequest
     for _ in range(12):  # eager, then replayed steps between the verified ones
         verify([Request("b", 4, [5, 6], b)])
         assert sample() == -1
@@ -279,7 +277,6 @@ def test_forward_refusals():
 def test_any_program_of_forks_steps_drafts_and_compactions(kv, kv_heads, d, seed):
     """Random calls; in the end every window holds the keys and values of its own tokens, as a session
     that was prefilled with them has them."""
-    from mesh_amd import DecodeMicrobatchRequest
     ctx = model_context(kv, 4, kv_heads, d, pages=220)
     rng = np.random.default_rng(seed)
     live = []  # [session, its tokens]
