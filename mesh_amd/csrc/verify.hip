@@ -22,7 +22,7 @@
 // of 64 x 5 rows x 128256, in f32 at the rate of the bytes).
 //
 // Three launches (us of 64 sequences with 4 drafts of 128256 columns, of one with 4
-// of 32000, measured one after another):
+// of 32000, measured one after another; the latter's last two are one of 11.6):
 //   verify_stats_kernel  one pass over all logits: per chunk of a row its largest
 //                        logit, the first place of it, and the f32 sum of weights
 //                        relative to it.  HBM bound (27.5: 6 TB/s; 3.6).
@@ -63,6 +63,7 @@ struct VerifyBufs {
     struct ChunkStat* stat;  // [rows][chunks]
     struct RestSum* rest;    // [n][rest_chunks]
     struct Decision* dec;    // [n]
+    int* done;               // [n] workgroups of a sequence that have their sums (0 between calls)
     int rest_chunks;
     uint32_t* out;
     int out_stride;
@@ -330,16 +331,131 @@ template <int N> __device__ inline Decision decide(const VerifyBufs& b, const Ve
             b.u[row0 + k], d0, a};
 }
 
+// Finds the token of a sequence by a workgroup of THREADS (mine: the chunk sums of
+// this lane's first chunk) and writes what the sequence comes to.  A chain of
+// latencies: what can be loaded before the decision is known is.
+template <int THREADS>
+__device__ inline void draw(const VerifyBufs& b, int s, const Decision& d, const RestSum* rs, const RestSum mine) {
+    __shared__ double sw[THREADS / 64];
+    __shared__ double s_before, s_target, s_z;
+    __shared__ int s_chunk, s_first, s_last;
+    __shared__ bool s_whole;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t y = tid < d.accepted ? b.drafts[d.first + tid] : 0;  // (at most 255 drafts)
+    uint32_t token = (uint32_t)d.at;
+    if (d.t > 0.0f && d.z > 0.0f) {
+        const float* xr = b.logits + (size_t)d.row * b.cols;
+        const float* qr = d.probs >= 0 ? b.probs + (size_t)d.probs * b.cols : nullptr;
+        const Weigher weight(d.m, d.t);
+        if (wave == 0) {
+            auto sum_of = [&](int c) { return c < 64 ? mine : rs[c]; };
+            double z = 0.0, total = 0.0;
+            for (int c = lane; c < b.rest_chunks; c += 64) z += sum_of(c).w;
+            z = wave_sum(z);
+            bool whole = false;  // the rest weighs nothing (by rounding): the token comes from p
+            auto chunk_sum = [&](int c) {
+                const RestSum x = sum_of(c);
+                return whole ? x.w : qr ? __builtin_fmax(__builtin_fma(-x.qa, z, x.wa), 0.0) : x.wa;
+            };
+            for (int pass = 0; pass < 2; ++pass) {
+                total = 0.0;
+                for (int c = lane; c < b.rest_chunks; c += 64) total += chunk_sum(c);
+                total = wave_sum(total);
+                if (total > 0.0) break;
+                whole = true;
+            }
+            const double target = (double)d.u * total;
+            // the first chunk whose end exceeds the target; none (u >= 1 or not a number): the last that weighs
+            double before = 0.0, pick_before = 0.0;
+            int chunk = 0;
+            bool found = false;
+            for (int c0 = 0; c0 < b.rest_chunks && !found; c0 += 64) {
+                const double w = c0 + lane < b.rest_chunks ? chunk_sum(c0 + lane) : 0.0;
+                const double run = wave_scan(w, lane);
+                const unsigned long long hit = __ballot(w > 0.0 && before + run > target), some = __ballot(w > 0.0);
+                if (some) {
+                    const int pick = hit ? __ffsll(hit) - 1 : 63 - __clzll(some);
+                    chunk = c0 + pick;
+                    pick_before = before + (pick ? lane_of(run, pick - 1) : 0.0);
+                    found = hit != 0;
+                }
+                before += lane_of(run, 63);
+            }
+            if (lane == 0) {
+                s_chunk = chunk;
+                s_before = pick_before;
+                s_target = target;
+                s_z = z;
+                s_whole = whole;
+                s_first = 0x7fffffff;
+                s_last = -1;
+            }
+        }
+        __syncthreads();
+        // the chunk's columns, E to a thread, in order
+        constexpr int E = kRestChunk / THREADS;
+        const int c0 = s_chunk * kRestChunk + tid * E;
+        const double z = s_z;
+        const bool whole = s_whole;
+        float x[E], q[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = c0 + e < b.cols ? xr[c0 + e] : -INFINITY;
+            q[e] = qr && c0 + e < b.cols ? fmaxf(qr[c0 + e], 0.0f) : 0.0f;
+        }
+        double w[E], sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            w[e] = weight.inf ? (x[e] == d.m ? 1.0 : 0.0) : weight(x[e]);
+            if (!whole) w[e] = qr ? __builtin_fmax(w[e] - (double)q[e] * z, 0.0) : (uint32_t)(c0 + e) == d.out ? 0.0 : w[e];
+            sum += w[e];
+        }
+        const double run = wave_scan(sum, lane);
+        if (lane == 63) sw[wave] = run;
+        __syncthreads();
+        double cum = s_before;
+        for (int i = 0; i < wave; ++i) cum += sw[i];
+        cum += run - sum;
+        int first = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            cum += w[e];
+            if (w[e] > 0.0) {
+                last = c0 + e;
+                if (first == 0x7fffffff && cum > s_target) first = c0 + e;
+            }
+        }
+        // (a wave's columns ascend with its lanes; one atomic a wave: every lane's own took 5 us)
+        const unsigned long long hit = __ballot(first != 0x7fffffff), some = __ballot(last >= 0);
+        if (hit && lane == __ffsll(hit) - 1) atomicMin(&s_first, first);
+        if (some && lane == 63 - __clzll(some)) atomicMax(&s_last, last);
+        __syncthreads();
+        // (no crossing: the chunk's sum and this one's order differ in their last bits, or u >= 1)
+        token = s_first != 0x7fffffff ? (uint32_t)s_first : s_last >= 0 ? (uint32_t)s_last : (uint32_t)d.at;
+    }
+    for (int i = tid; i < b.out_stride; i += THREADS)
+        b.out[(size_t)s * b.out_stride + i] = i < d.accepted ? y : i == d.accepted ? token : 0xffffffffu;
+    if (tid == 0) b.accepted[s] = d.accepted;
+}
+
 // A workgroup takes `per` chunks of one sequence's emission row in turn: as many as
 // leave no more workgroups than the chip holds at once, for each has the tests to do first.
-template <int N>
+// DRAW: few workgroups in all; the last of a sequence's draws its token as well, and
+// a third launch is saved.  It knows that it is by a count (its own chunk sums are
+// released by its addition to it, the others' acquired with it); many workgroups would
+// pay a write-back of an XCD's L2 each.
+template <int N, bool DRAW>
 __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyArgs<N> v, int per, int groups) {
     __shared__ double ss[2][3][4];
     constexpr int E = kRestChunk / 256;
     const int s = blockIdx.x / groups, g = blockIdx.x - s * groups, tid = threadIdx.x;
     const Decision d = decide(b, v, s);
-    if (g == 0 && tid == 0) b.dec[s] = d;
-    if (d.t <= 0.0f || d.z <= 0.0f) return;  // greedy, or nothing weighs: the first largest logit
+    RestSum* rs = b.rest + (size_t)s * b.rest_chunks;
+    if (!DRAW && g == 0 && tid == 0) b.dec[s] = d;
+    if (d.t <= 0.0f || d.z <= 0.0f) {  // greedy, or nothing weighs: the first largest logit
+        if (DRAW && g == 0) draw<256>(b, s, d, rs, RestSum{});
+        return;
+    }
     const float* xr = b.logits + (size_t)d.row * b.cols;
     const float* qr = d.probs >= 0 ? b.probs + (size_t)d.probs * b.cols : nullptr;
     const Weigher weight(d.m, d.t);
@@ -393,122 +509,39 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyBufs b, VerifyAr
             double o[3];
 #pragma unroll
             for (int i = 0; i < 3; ++i) o[i] = (ss[buf][i][0] + ss[buf][i][1]) + (ss[buf][i][2] + ss[buf][i][3]);
-            b.rest[(size_t)s * b.rest_chunks + ch] = {o[0], o[1], o[2]};
+            rs[ch] = {o[0], o[1], o[2]};
         }
+    }
+    if constexpr (DRAW) {
+        __shared__ bool s_mine;
+        if (tid == 0) {
+            const int before = __hip_atomic_fetch_add(b.done + s, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            s_mine = before == groups - 1;
+            if (s_mine) b.done[s] = 0;  // for the next call
+        }
+        __syncthreads();
+        if (!s_mine) return;
+        draw<256>(b, s, d, rs, rs[min(tid & 63, b.rest_chunks - 1)]);
     }
 }
 
-// A workgroup of 16 waves per sequence.  A chain of latencies: what can be loaded
-// before the decision is known is, and two columns a thread keep the code short
+// A workgroup of 16 waves per sequence: two columns a thread keep the code short
 // (its first pass waits for every line of it).
 constexpr int kEmitThreads = 1024;
 __global__ __launch_bounds__(kEmitThreads) void verify_emit_kernel(VerifyBufs b) {
-    __shared__ double sw[kEmitThreads / 64];
-    __shared__ double s_before, s_target, s_z;
-    __shared__ int s_chunk, s_first, s_last;
-    __shared__ bool s_whole;
-    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int s = blockIdx.x;
     const RestSum* rs = b.rest + (size_t)s * b.rest_chunks;
-    const RestSum mine = rs[min(lane, b.rest_chunks - 1)];  // the lane's first chunk (of a greedy row: not used)
+    const RestSum mine = rs[min((int)(threadIdx.x & 63), b.rest_chunks - 1)];  // (of a greedy row: not used)
     const Decision d = b.dec[s];
-    const uint32_t y = tid < d.accepted ? b.drafts[d.first + tid] : 0;  // (at most 255 drafts)
-    uint32_t token = (uint32_t)d.at;
-    if (d.t > 0.0f && d.z > 0.0f) {
-        const float* xr = b.logits + (size_t)d.row * b.cols;
-        const float* qr = d.probs >= 0 ? b.probs + (size_t)d.probs * b.cols : nullptr;
-        const Weigher weight(d.m, d.t);
-        if (wave == 0) {
-            auto sum_of = [&](int c) { return c < 64 ? mine : rs[c]; };
-            double z = 0.0, total = 0.0;
-            for (int c = lane; c < b.rest_chunks; c += 64) z += sum_of(c).w;
-            z = wave_sum(z);
-            bool whole = false;  // the rest weighs nothing (by rounding): the token comes from p
-            auto chunk_sum = [&](int c) {
-                const RestSum x = sum_of(c);
-                return whole ? x.w : qr ? __builtin_fmax(__builtin_fma(-x.qa, z, x.wa), 0.0) : x.wa;
-            };
-            for (int pass = 0; pass < 2; ++pass) {
-                total = 0.0;
-                for (int c = lane; c < b.rest_chunks; c += 64) total += chunk_sum(c);
-                total = wave_sum(total);
-                if (total > 0.0) break;
-                whole = true;
-            }
-            const double target = (double)d.u * total;
-            // the first chunk whose end exceeds the target; none (u >= 1 or not a number): the last that weighs
-            double before = 0.0, pick_before = 0.0;
-            int chunk = 0;
-            bool found = false;
-            for (int c0 = 0; c0 < b.rest_chunks && !found; c0 += 64) {
-                const double w = c0 + lane < b.rest_chunks ? chunk_sum(c0 + lane) : 0.0;
-                const double run = wave_scan(w, lane);
-                const unsigned long long hit = __ballot(w > 0.0 && before + run > target), some = __ballot(w > 0.0);
-                if (some) {
-                    const int pick = hit ? __ffsll(hit) - 1 : 63 - __clzll(some);
-                    chunk = c0 + pick;
-                    pick_before = before + (pick ? lane_of(run, pick - 1) : 0.0);
-                    found = hit != 0;
-                }
-                before += lane_of(run, 63);
-            }
-            if (lane == 0) {
-                s_chunk = chunk;
-                s_before = pick_before;
-                s_target = target;
-                s_z = z;
-                s_whole = whole;
-                s_first = 0x7fffffff;
-                s_last = -1;
-            }
-        }
-        __syncthreads();
-        // the chunk's columns, E to a thread, in order
-        constexpr int E = kRestChunk / kEmitThreads;
-        const int c0 = s_chunk * kRestChunk + tid * E;
-        const double z = s_z;
-        const bool whole = s_whole;
-        float x[E], q[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] = c0 + e < b.cols ? xr[c0 + e] : -INFINITY;
-            q[e] = qr && c0 + e < b.cols ? fmaxf(qr[c0 + e], 0.0f) : 0.0f;
-        }
-        double w[E], sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            w[e] = weight.inf ? (x[e] == d.m ? 1.0 : 0.0) : weight(x[e]);
-            if (!whole) w[e] = qr ? __builtin_fmax(w[e] - (double)q[e] * z, 0.0) : (uint32_t)(c0 + e) == d.out ? 0.0 : w[e];
-            sum += w[e];
-        }
-        const double run = wave_scan(sum, lane);
-        if (lane == 63) sw[wave] = run;
-        __syncthreads();
-        double cum = s_before;
-        for (int i = 0; i < wave; ++i) cum += sw[i];
-        cum += run - sum;
-        int first = 0x7fffffff, last = -1;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            cum += w[e];
-            if (w[e] > 0.0) {
-                last = c0 + e;
-                if (first == 0x7fffffff && cum > s_target) first = c0 + e;
-            }
-        }
-        // (a wave's columns ascend with its lanes; one atomic a wave: every lane's own took 5 us)
-        const unsigned long long hit = __ballot(first != 0x7fffffff), some = __ballot(last >= 0);
-        if (hit && lane == __ffsll(hit) - 1) atomicMin(&s_first, first);
-        if (some && lane == 63 - __clzll(some)) atomicMax(&s_last, last);
-        __syncthreads();
-        // (no crossing: the chunk's sum and this one's order differ in their last bits, or u >= 1)
-        token = s_first != 0x7fffffff ? (uint32_t)s_first : s_last >= 0 ? (uint32_t)s_last : (uint32_t)d.at;
-    }
-    for (int i = tid; i < b.out_stride; i += kEmitThreads)
-        b.out[(size_t)s * b.out_stride + i] = i < d.accepted ? y : i == d.accepted ? token : 0xffffffffu;
-    if (tid == 0) b.accepted[s] = d.accepted;
+    draw<kEmitThreads>(b, s, d, rs, mine);
 }
 
-// The pass over all logits and that over the emission rows of m <= N sequences.
+// Workgroups up to which the rest's kernel draws too (us a call, three launches / two:
+// 16 workgroups 13.7 / 10.5, 63 13.0 / 11.6, 64 12.2 / 11.6, 126 12.5 / 14.6, 128 12.2 /
+// 13.3, 504 14.6 / 23.4, 1008 18.3 / 41.9).
+constexpr int kDrawWgs = 64;
+
+// The launches of m <= N sequences.
 template <int N>
 void launch_passes(zr_context* ctx, const VerifyBufs& b, const int* draft_len, const float* temperature, int m, int e) {
     VerifyArgs<N> v;
@@ -529,7 +562,15 @@ void launch_passes(zr_context* ctx, const VerifyBufs& b, const int* draft_len, c
         default: stats(verify_stats_kernel<8, N>); break;
     }
     const int per = (m * b.rest_chunks + 2047) / 2048, groups = (b.rest_chunks + per - 1) / per;
-    hipLaunchKernelGGL(verify_rest_kernel<N>, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
+    auto rest = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(m * groups), dim3(256), 0, ctx->stream, b, v, per, groups);
+    };
+    if (m * groups <= kDrawWgs) {
+        rest(verify_rest_kernel<N, true>);
+    } else {
+        rest(verify_rest_kernel<N, false>);
+        hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(kEmitThreads), 0, ctx->stream, b);
+    }
 }
 
 }  // namespace
@@ -546,7 +587,8 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
     while (e > 1 && rows * ((cols + 1024 * e - 1) / (1024 * e)) < 1024) e /= 2;
     const int chunk = 1024 * e, chunks = (cols + chunk - 1) / chunk;
     const int rest_chunks = (cols + kRestChunk - 1) / kRestChunk;
-    const size_t stat_bytes = sizeof(ChunkStat) * (size_t)rows * chunks;
+    constexpr size_t done_bytes = sizeof(int) * kSeqs;  // (first, whatever the call: 0 between calls)
+    const size_t stat_bytes = done_bytes + sizeof(ChunkStat) * (size_t)rows * chunks;
     const size_t dec_bytes = sizeof(Decision) * (size_t)n, need = stat_bytes + dec_bytes + sizeof(RestSum) * (size_t)n * rest_chunks;
     if (need > ctx->verify_ws_bytes) {
         ZR_HIP(ctx, hipStreamSynchronize(ctx->stream));
@@ -557,6 +599,7 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
         if (err != hipSuccess)
             return set_err(ctx, err == hipErrorOutOfMemory ? ZR_E_OOM : ZR_E_HIP, "verification workspace of %zu bytes: %s",
                            need, hipGetErrorString(err));
+        ZR_HIP(ctx, hipMemsetAsync(ctx->verify_ws, 0, done_bytes, ctx->stream));
         ctx->verify_ws_bytes = need;
     }
     hipEvent_t ev;
@@ -574,7 +617,8 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
         b.drafts = vb->d_drafts + draft0;
         b.probs = vb->d_draft_probs ? vb->d_draft_probs + draft0 * cols : nullptr;
         b.u = vb->d_uniforms + row0;
-        b.stat = (ChunkStat*)ctx->verify_ws + row0 * chunks;
+        b.done = (int*)ctx->verify_ws;
+        b.stat = (ChunkStat*)((char*)ctx->verify_ws + done_bytes) + row0 * chunks;
         b.dec = (Decision*)((char*)ctx->verify_ws + stat_bytes) + s0;
         b.rest = (RestSum*)((char*)ctx->verify_ws + stat_bytes + dec_bytes) + (size_t)s0 * rest_chunks;
         b.rest_chunks = rest_chunks;
@@ -587,8 +631,6 @@ zr_status launch_verify(zr_context* ctx, const float* d_logits, int cols, const 
             launch_passes<kFewSeqs>(ctx, b, lens, temps, m, e);
         else
             launch_passes<kSeqs>(ctx, b, lens, temps, m, e);
-        ZR_LAUNCH_CHECK(ctx);
-        hipLaunchKernelGGL(verify_emit_kernel, dim3(m), dim3(kEmitThreads), 0, ctx->stream, b);
         ZR_LAUNCH_CHECK(ctx);
         row0 += r;
         draft0 += r - m;

@@ -282,3 +282,19 @@ def test_rows_at_any_alignment(ctx, cols, x_off, q_off):
     assert a.tolist() == want[1]
     for s in range(3):
         assert t[s, :a[s] + 1].tolist() == want[0][s] and np.all(t[s, a[s] + 1:] == 0xffffffff)
+
+
+@pytest.mark.parametrize("certain", [False, True])
+def test_small_calls_draw_in_two_launches_again_and_again(ctx, certain):
+    """Calls of 1 to 64 workgroups over the emission rows, and one above, in turn: the count of a
+    sequence's workgroups is back at 0 behind every call, also where a row is greedy."""
+    rng = np.random.default_rng(31)
+    sets = []
+    for lens, cols in (([4], 32000), ([2], 2048), ([1, 3, 0], 40000), ([2] * 32, 4000), ([3, 1], 66000), ([4, 0, 2], 60000)):
+        temps = np.where(rng.random(len(lens)) < 0.25, 0.0, 0.9).astype(np.float32)
+        p = problem(rng, cols, lens, temps, certain)
+        sets.append((p, temps, expect(p[0], p[1], temps, p[2], p[3])))
+    for _ in range(3):
+        for i in rng.permutation(len(sets)):
+            (logits, drafts, u, q), temps, want = sets[i]
+            assert verify_device(ctx, logits, drafts, temps, u, q) == want
